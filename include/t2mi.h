@@ -91,6 +91,9 @@ const char* t2_last_error(void);
 
 /* One context per GPU per thread.  hip_stream may be NULL (the library creates its own stream). */
 int t2_ctx_create(int device, void* hip_stream, t2_ctx** out);
+/* A context that enqueues on hip_stream itself, whatever it is: NULL is the device's default stream.  For callers whose other
+ * work runs on that stream already: nothing has to be ordered against it.  The library never destroys the stream. */
+int t2_ctx_create_on_stream(int device, void* hip_stream, t2_ctx** out);
 int t2_ctx_destroy(t2_ctx* ctx);
 int t2_ctx_synchronize(t2_ctx* ctx);
 

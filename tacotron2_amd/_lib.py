@@ -51,6 +51,7 @@ _SIGS = {
     "t2_version": (C.c_int, []),
     "t2_last_error": (C.c_char_p, []),
     "t2_ctx_create": (C.c_int, [C.c_int, _p, C.POINTER(_p)]),
+    "t2_ctx_create_on_stream": (C.c_int, [C.c_int, _p, C.POINTER(_p)]),
     "t2_ctx_destroy": (C.c_int, [_p]),
     "t2_ctx_synchronize": (C.c_int, [_p]),
     "t2_model_create": (C.c_int, [_p, C.POINTER(T2Dims), C.POINTER(_p)]),

@@ -13,6 +13,7 @@
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+#include "rng.h"
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -46,20 +47,6 @@ __host__ __device__ inline size_t frag_idx(int row, int k, int MB) {
 
 __device__ __forceinline__ float sigmoidf_(float x) { return 1.0f / (1.0f + expf(-x)); }
 
-// Counter-based generator of the sampled training paths (PreNet / conv dropout, zoneout): 24 uniform bits per
-// (seed, stream, step, row, column).  TensorFlow's stateful random ops cannot be reproduced; the oracle uses this same
-// function (oracle/t2_oracle.py:rng_u01), TF's arithmetic around it.
-__host__ __device__ inline uint32_t t2_mix32(uint32_t x) {
-    x ^= x >> 16; x *= 0x7FEB352Du; x ^= x >> 15; x *= 0x846CA68Bu; x ^= x >> 16;
-    return x;
-}
-__host__ __device__ inline float t2_u01(uint32_t seed, uint32_t stream, uint32_t t, uint32_t row, uint32_t col) {
-    uint32_t h = t2_mix32(seed ^ (stream * 0x9E3779B9u));
-    h = t2_mix32(h ^ (t * 0x85EBCA6Bu + 0x165667B1u));
-    h = t2_mix32(h ^ (row * 0xC2B2AE35u + 0x27D4EB2Fu));
-    h = t2_mix32(h ^ (col * 0x9E3779B1u + 0x85EBCA77u));
-    return (float)(h >> 8) * (1.0f / 16777216.0f);
-}
 // tf.nn.dropout(x, keep_prob) of TF 1.11/1.12: x / keep_prob * floor(keep_prob + uniform)
 __device__ __forceinline__ float dropout_train(float x, float rate, float u) { return (u >= rate) ? x / (1.0f - rate) : 0.0f; }
 #define T2_STREAM_PRENET 1

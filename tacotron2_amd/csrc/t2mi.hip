@@ -1,7 +1,7 @@
 // libt2mi.so -- host side of the C-ABI declared in include/t2mi.h.
 // Weight repacking, workspaces, launch sequences (eager or hipGraph-chunked) for the kernels in
 // kernels.h.  No CPU fallback: every entry point runs HIP kernels or fails.
-#include "../../include/t2mi.h"
+#include "ctx.h"
 #include "kernels.h"
 #include "persist.h"
 #include "persist_bwd.h"
@@ -13,6 +13,7 @@
 #include <cstring>
 #include <map>
 #include <mutex>
+#include <new>
 #include <string>
 #include <utility>
 #include <vector>
@@ -22,7 +23,7 @@
 // ------------------------------------------------------------------------------------------------
 static thread_local char g_err[512] = "";
 
-static int fail(int code, const char* fmt, ...) {
+int fail(int code, const char* fmt, ...) {
     va_list ap;
     va_start(ap, fmt);
     vsnprintf(g_err, sizeof(g_err), fmt, ap);
@@ -30,35 +31,12 @@ static int fail(int code, const char* fmt, ...) {
     return code;
 }
 
-#define HIP_TRY(expr)                                                                              \
-    do {                                                                                           \
-        hipError_t e_ = (expr);                                                                    \
-        if (e_ != hipSuccess)                                                                      \
-            return fail(e_ == hipErrorOutOfMemory ? T2_ENOMEM : T2_EHIP, "%s failed: %s (%s:%d)", #expr, \
-                        hipGetErrorString(e_), __FILE__, __LINE__);                                \
-    } while (0)
-
-#define T2_TRY(expr)              \
-    do {                          \
-        int r_ = (expr);          \
-        if (r_ != T2_OK) return r_; \
-    } while (0)
-
 extern "C" int t2_version(void) { return T2_ABI_VERSION; }
 extern "C" const char* t2_last_error(void) { return g_err; }
 
 // ------------------------------------------------------------------------------------------------
 // handles
 // ------------------------------------------------------------------------------------------------
-struct t2_ctx {
-    int device;
-    hipStream_t stream;
-    bool own_stream;
-    float* red_ws = nullptr;   // partial sums of the loss reductions (train.h)
-    void* voc_ws = nullptr;    // Griffin-Lim workspace (vocoder.h), grown on demand
-    size_t voc_ws_bytes = 0;
-};
-
 struct HostWeight {
     std::vector<float> data;
     std::vector<int64_t> shape;
@@ -378,7 +356,7 @@ static int make_conv(t2_model* m, ConvLayer* L, const std::string& prefix, int k
 // ctx / model
 // ------------------------------------------------------------------------------------------------
 static int noalloc_setup(int device);     // train.h
-extern "C" int t2_ctx_create(int device, void* hip_stream, t2_ctx** out) {
+static int ctx_create(int device, hipStream_t stream, bool own, t2_ctx** out) {
     if (!out) return fail(T2_EINVAL, "out is null");
     int n = 0;
     HIP_TRY(hipGetDeviceCount(&n));
@@ -389,18 +367,25 @@ extern "C" int t2_ctx_create(int device, void* hip_stream, t2_ctx** out) {
     if (strncmp(prop.gcnArchName, "gfx950", 6) != 0)
         return fail(T2_EHIP, "device %d is %s; libt2mi is built for gfx950 only", device, prop.gcnArchName);
     T2_TRY(noalloc_setup(device));        // per-device address of the allocation-free entry point's scratch array (train.h)
-    t2_ctx* c = new t2_ctx();
+    t2_ctx* c = new (std::nothrow) t2_ctx();
+    if (!c) return fail(T2_ENOMEM, "out of host memory");
     c->device = device;
-    if (hip_stream) {
-        c->stream = (hipStream_t)hip_stream;
-        c->own_stream = false;
-    } else {
+    c->stream = stream;
+    c->own_stream = own;
+    if (own) {
         hipError_t e = hipStreamCreateWithFlags(&c->stream, hipStreamNonBlocking);
         if (e != hipSuccess) { delete c; return fail(T2_EHIP, "hipStreamCreate failed: %s", hipGetErrorString(e)); }
-        c->own_stream = true;
     }
     *out = c;
     return T2_OK;
+}
+
+extern "C" int t2_ctx_create(int device, void* hip_stream, t2_ctx** out) {
+    return ctx_create(device, (hipStream_t)hip_stream, hip_stream == nullptr, out);
+}
+
+extern "C" int t2_ctx_create_on_stream(int device, void* hip_stream, t2_ctx** out) {
+    return ctx_create(device, (hipStream_t)hip_stream, false, out);
 }
 
 extern "C" int t2_ctx_destroy(t2_ctx* c) {

@@ -9,6 +9,7 @@ from __future__ import annotations
 import contextlib
 import ctypes as C
 import os
+import threading
 import weakref
 from typing import Dict, Optional
 
@@ -134,6 +135,40 @@ def shared_context(device: int = 0) -> Context:
     if device not in _shared:
         _shared[device] = Context(device)
     return _shared[device]
+
+
+class StreamContext(Context):
+    """A context on a stream of the caller's: the library enqueues where the caller's other work is, and ``ordered`` has nothing
+    to order.  Creating one leaves torch's current device as it was."""
+
+    def __init__(self, device: int, stream: torch.cuda.Stream):
+        self.lib = _lib.load()
+        self.device = torch.device("cuda", device)
+        self.stream = stream
+        self.handle = C.c_void_p()
+        with torch.cuda.device(self.device):
+            _lib.check(self.lib.t2_ctx_create_on_stream(device, C.c_void_p(stream.cuda_stream), C.byref(self.handle)))
+
+    @contextlib.contextmanager
+    def ordered(self):
+        yield
+
+
+_on_stream: Dict[tuple, StreamContext] = {}
+
+
+def stream_context(device: Optional[int] = None) -> StreamContext:
+    """The context of torch's current stream on ``device`` (default: the current device).  It holds no workspace, so it serves
+    the entry points that take theirs from the caller (recurrence, AdamW)."""
+    if not torch.cuda.is_available():
+        raise RuntimeError("tacotron2_amd needs an MI355X (gfx950) GPU: there is no CPU path")
+    if device is None:
+        device = torch.cuda.current_device()
+    stream = torch.cuda.current_stream(device)
+    key = (device, stream.cuda_stream, threading.get_ident())
+    if key not in _on_stream:
+        _on_stream[key] = StreamContext(device, stream)
+    return _on_stream[key]
 
 
 class Engine:

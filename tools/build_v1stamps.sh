@@ -3,6 +3,7 @@
 set -euo pipefail
 cd "$(dirname "$0")/.."
 mkdir -p tools/bin
-/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -shared -Wno-unused-function -Wno-unused-value -DV1D_STAMPS \
+/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -shared -Wno-unused-function -Wno-unused-value \
+    -Xclang -target-feature -Xclang -packed-fp32-ops -DV1D_STAMPS \
     -o tools/bin/libt2mi_v1stamps.so tacotron2_amd/csrc/t2mi.hip
 echo built tools/bin/libt2mi_v1stamps.so

@@ -1,5 +1,5 @@
 // Micro-benchmark of the conv GEMM fast path at PostNetV2's shape (not part of the library).
-// Build: hipcc --offload-arch=gfx950 -O3 -std=c++17 tools/conv_bench.hip -o /tmp/conv_bench
+// Build: hipcc --offload-arch=gfx950 -O3 -std=c++17 -Xclang -target-feature -Xclang -packed-fp32-ops tools/conv_bench.hip -o /tmp/conv_bench
 #include "../tacotron2_amd/csrc/kernels.h"
 #include <cstdio>
 #include <cstdlib>

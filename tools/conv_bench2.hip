@@ -1,5 +1,5 @@
 // Experiment bench of the conv GEMM forward fast path (not part of the library): variants of conv_gemm_kt_kernel (kernels.h).
-// Build: hipcc --offload-arch=gfx950 -O3 -std=c++17 tools/conv_bench2.hip -o tools/bin/conv_bench2
+// Build: hipcc --offload-arch=gfx950 -O3 -std=c++17 -Xclang -target-feature -Xclang -packed-fp32-ops tools/conv_bench2.hip -o tools/bin/conv_bench2
 #include "../tacotron2_amd/csrc/kernels.h"
 template <int NS, int WN, int ORDER>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(WN == 4 ? 3 : 2, WN == 4 ? 3 : 4)))

@@ -1,5 +1,5 @@
 // Micro-benchmark / ablation harness for lstm_step_kernel (not part of the library).
-// Build: hipcc --offload-arch=gfx950 -O3 -std=c++17 [-DT2_ABL_NOA] [-DT2_ABL_NOW] [-DT2_ABL_NOMMA] tools/lstm_bench.hip -o /tmp/lstm_bench
+// Build: hipcc --offload-arch=gfx950 -O3 -std=c++17 -Xclang -target-feature -Xclang -packed-fp32-ops [-DT2_ABL_NOA] [-DT2_ABL_NOW] [-DT2_ABL_NOMMA] tools/lstm_bench.hip -o /tmp/lstm_bench
 #include "../tacotron2_amd/csrc/kernels.h"
 #include <cstdio>
 #include <cstdlib>
