@@ -428,6 +428,50 @@ int t2v1_train_decoder_backward(t2v1_dtrainer* tr, const float* done, const floa
 int t2_griffin_lim(t2_ctx* ctx, const float* spectrogram, int B, int T, int num_freq, int win_length, int hop_length,
                    float min_level_db, float ref_level_db, float power, int iters, float* wav);
 
+/* ---- gated linear recurrence (no counterpart in the reference; beside ZoneoutLSTMCell, tacotron/modules.py:235-283, and GRUCell) ----
+ * For every row b and channel c, over the row's positions in order (from the last to the first where `reverse` is set):
+ *     a = sigmoid(f_t)      h_t = a h_{t-1} + (1 - a) z_t      y_t = sigmoid(o_t) h_t   (y_t = h_t where o is NULL)
+ * The recurrence is linear in h, so a whole sequence is a scan: it is split over the time axis, not run step by step.
+ *  - z, f, o, y: [B][T][H] of one type, channels contiguous, strides in elements (any, 0 for inputs that are broadcast); o may be NULL.
+ *    y must not overlap an input or itself.
+ *  - lens: dev int64 [B] or NULL (all T).  Values outside [0, T] are taken as 0 and T.  Positions at or behind a row's length are not
+ *    read into any result and give y = 0; a length of 0 leaves the state as it was.
+ *  - state, final_state: dev fp32 [B][H] or NULL (zeros / not wanted).  They may be the same buffer.
+ *  - tape: dev fp32 of t2_gated_scan_tape() floats or NULL.  The forward call fills it with the state in front of every
+ *    T2_SCAN_SPAN-th step; t2_gated_scan_backward recomputes the rest from there.
+ *  - ws: dev buffer of t2_gated_scan_ws() bytes, 16-byte aligned, used by this call only (no content is kept between calls: two captured
+ *    graphs that may run at once need a buffer each).
+ * Gates, state and sums are fp32 whatever the type; y and the gradients are rounded once.
+ * t2_gated_scan_backward: dy [B][T][H] of the same type, dfinal dev fp32 [B][H] or NULL (the gradient of final_state) ->
+ *     dz, df, do (do where o was given), dstate (dev fp32 [B][H] or NULL); zeros at positions behind a row's length.
+ * t2_gated_scan_step: one new position for each row, z, f, o, y [B][H] (stride_b only), state dev fp32 [B][H] with a row stride, updated in place.
+ *     active: dev uint8 [B] or NULL; rows where it is 0 keep their state and get y = 0.
+ * All three only enqueue; none allocates, so they can be captured. */
+#define T2_F32 0
+#define T2_BF16 1
+#define T2_F16 2
+#define T2_SCAN_SPAN 64
+typedef struct t2_seq { const void* ptr; int64_t stride_b, stride_t; } t2_seq;
+typedef struct t2_scan_args {
+    int32_t dtype, B, T, H, reverse;
+    t2_seq z, f, o, y;            /* y: written by the forward call and by the step                            */
+    const int64_t* lens;
+    const float* state;           /* backward: the state the forward call was given                            */
+    float* final_state;
+    float* tape;
+    t2_seq dy, dz, df, do_;       /* backward only                                                             */
+    const float* dfinal;
+    float* dstate;
+    void* ws;
+    int64_t ws_bytes;
+} t2_scan_args;
+int64_t t2_gated_scan_tape(int B, int T, int H);                 /* floats; < 0: T2_EINVAL */
+int64_t t2_gated_scan_ws(int B, int T, int H);                   /* bytes of the forward or the backward call, 0: none needed */
+int t2_gated_scan(t2_ctx* ctx, const t2_scan_args* a);
+int t2_gated_scan_backward(t2_ctx* ctx, const t2_scan_args* a);
+int t2_gated_scan_step(t2_ctx* ctx, int dtype, int B, int H, const void* z, int64_t z_stride, const void* f, int64_t f_stride, const void* o,
+                       int64_t o_stride, float* state, int64_t state_stride, const uint8_t* active, void* y, int64_t y_stride);
+
 #ifdef __cplusplus
 }
 #endif

@@ -38,6 +38,24 @@ class T2V1Dims(C.Structure):
     ]
 
 
+T2_F32, T2_BF16, T2_F16 = 0, 1, 2
+T2_SCAN_SPAN = 64
+
+
+class T2Seq(C.Structure):
+    _fields_ = [("ptr", C.c_void_p), ("stride_b", C.c_int64), ("stride_t", C.c_int64)]
+
+
+class T2ScanArgs(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("B", C.c_int32), ("T", C.c_int32), ("H", C.c_int32), ("reverse", C.c_int32),
+        ("z", T2Seq), ("f", T2Seq), ("o", T2Seq), ("y", T2Seq),
+        ("lens", C.c_void_p), ("state", C.c_void_p), ("final_state", C.c_void_p), ("tape", C.c_void_p),
+        ("dy", T2Seq), ("dz", T2Seq), ("df", T2Seq), ("do_", T2Seq), ("dfinal", C.c_void_p), ("dstate", C.c_void_p),
+        ("ws", C.c_void_p), ("ws_bytes", C.c_int64),
+    ]
+
+
 class T2Error(RuntimeError):
     def __init__(self, code, msg):
         super().__init__(f"libt2mi error {code}: {msg}")
@@ -132,6 +150,14 @@ _SIGS = {
     "t2_optim_set_state": (C.c_int, [_p, _p, _p, C.c_int64]),
     "t2_griffin_lim": (C.c_int, [_p, _p, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_float, C.c_float, C.c_float, C.c_int, _p]),
 }
+
+_SIGS.update({
+    "t2_gated_scan_tape": (C.c_int64, [C.c_int, C.c_int, C.c_int]),
+    "t2_gated_scan_ws": (C.c_int64, [C.c_int, C.c_int, C.c_int]),
+    "t2_gated_scan": (C.c_int, [_p, C.POINTER(T2ScanArgs)]),
+    "t2_gated_scan_backward": (C.c_int, [_p, C.POINTER(T2ScanArgs)]),
+    "t2_gated_scan_step": (C.c_int, [_p, C.c_int, C.c_int, C.c_int, _p, C.c_int64, _p, C.c_int64, _p, C.c_int64, _p, C.c_int64, _p, _p, C.c_int64]),
+})
 
 _lib = None
 

@@ -1,0 +1,181 @@
+"""Gated linear recurrence on the HIP library: whole sequences, their backward pass, and one position at a time.
+
+    a_t = sigmoid(f_t)      h_t = a_t h_{t-1} + (1 - a_t) z_t      y_t = sigmoid(o_t) h_t   (y_t = h_t without o)
+
+The gates do not depend on h, so a sequence is a scan that runs in parallel over time; the LSTM and GRU cells of
+``modules`` / ``rnn_impl`` need a hop for every step.  z, f and o are what a projection of the layer's input gives (slices of one
+[B, T, 3H] product need no copy).  fp32, bf16 and fp16; gates, state and sums are fp32, results are rounded once.
+
+``ctx`` is a Context, an Engine, or None: torch's current stream on the tensors' device.  Nothing here synchronises, and every
+call can be captured into a graph (lengths on the host cannot: they have to be copied first)."""
+from __future__ import annotations
+
+from typing import NamedTuple, Optional, Tuple
+
+import numpy as np
+import torch
+
+from . import _lib
+from .engine import Context, stream_context
+
+_DTYPES = {torch.float32: _lib.T2_F32, torch.bfloat16: _lib.T2_BF16, torch.float16: _lib.T2_F16}
+
+
+class ScanTape(NamedTuple):
+    """What ``gated_scan_backward`` needs of a forward call: its inputs (not copied: leave them as they are until then) and the
+    states in front of every 64th step."""
+    z: torch.Tensor
+    f: torch.Tensor
+    o: Optional[torch.Tensor]
+    lens: Optional[torch.Tensor]
+    reverse: bool
+    states: torch.Tensor
+
+
+def _context(ctx, t: torch.Tensor) -> Context:
+    if ctx is None:
+        return stream_context(t.device.index)
+    ctx = ctx if isinstance(ctx, Context) else ctx.context
+    if ctx.device != t.device:
+        raise ValueError(f"tensors on {t.device}, context on {ctx.device}")
+    return ctx
+
+
+def _sequence(what: str, t, like: Optional[torch.Tensor] = None) -> torch.Tensor:
+    if not (isinstance(t, torch.Tensor) and t.is_cuda):
+        raise ValueError(f"{what} must be a device tensor")
+    if like is None:
+        if t.dim() != 3 or t.dtype not in _DTYPES or 0 in t.shape:
+            raise ValueError(f"{what} must be a non-empty [B, T, H] tensor of float32, bfloat16 or float16, got {t.dtype} {tuple(t.shape)}")
+    elif t.shape != like.shape or t.dtype != like.dtype or t.device != like.device:
+        raise ValueError(f"{what} must be {like.dtype} {tuple(like.shape)} on {like.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    if t.shape[2] > 1 and t.stride(2) != 1:
+        raise ValueError(f"the channels of {what} must be contiguous")
+    return t
+
+
+def _output(what: str, t, like: torch.Tensor) -> torch.Tensor:
+    if t is None:
+        return torch.empty(like.shape, dtype=like.dtype, device=like.device)
+    _sequence(what, t, like)
+    B, T, H = t.shape
+    sb, st = t.stride(0), t.stride(1)
+    by_row = (T == 1 or st >= H) and (B == 1 or sb >= (T - 1) * st + H)
+    by_time = (B == 1 or sb >= H) and (T == 1 or st >= (B - 1) * sb + H)
+    if not (by_row or by_time):
+        raise ValueError(f"the elements of {what} overlap (strides {t.stride()})")
+    return t
+
+
+def _rows(what: str, t, B: int, H: int, device) -> torch.Tensor:
+    if not (isinstance(t, torch.Tensor) and t.device == device and t.dtype == torch.float32 and tuple(t.shape) == (B, H)):
+        raise ValueError(f"{what} must be a float32 [{B}, {H}] tensor on {device}")
+    return t.contiguous()
+
+
+def _lengths(lens, B: int, T: int, device) -> Optional[torch.Tensor]:
+    if lens is None:
+        return None
+    if isinstance(lens, torch.Tensor) and lens.is_cuda:
+        if tuple(lens.shape) != (B,) or lens.device != device or lens.dtype not in (torch.int64, torch.int32):
+            raise ValueError(f"lens must be an int64 or int32 [{B}] tensor on {device}")
+        return lens.to(torch.int64).contiguous()
+    host = np.asarray(lens)
+    if host.shape != (B,) or host.dtype.kind not in "iu" or (host < 0).any() or (host > T).any():
+        raise ValueError(f"lens must be {B} whole numbers from 0 to {T}")
+    return torch.from_numpy(host.astype(np.int64)).to(device)
+
+
+def _seq(t: Optional[torch.Tensor]):
+    return (None, 0, 0) if t is None else (t.data_ptr(), t.stride(0), t.stride(1))
+
+
+def _ptr(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+def _workspace(ctx: Context, B: int, T: int, H: int) -> Tuple[Optional[torch.Tensor], int]:
+    n = ctx.lib.t2_gated_scan_ws(B, T, H)
+    if n < 0:
+        _lib.check(_lib.T2_EINVAL)
+    return (torch.empty(n, dtype=torch.uint8, device=ctx.device), n) if n else (None, 0)
+
+
+def gated_scan(ctx, z, f, o=None, lens=None, state=None, reverse: bool = False, tape: bool = False, out=None):
+    """y [B, T, H] and the final state [B, H] (fp32) of the recurrence over z, f (and o) [B, T, H]; with ``tape`` also the ScanTape of
+    the backward pass.
+
+    Any batch and time strides (time-major views, slices of a projection, broadcast inputs), contiguous channels.  ``lens`` [B]: row b
+    has positions 0 .. lens[b] - 1; the others give y = 0 and do not touch the state.  Host lengths outside [0, T] raise, device
+    lengths are taken as the nearest.  ``reverse`` runs every row from its last position to its first.  ``state``: the state in
+    front of the first step (fp32 [B, H], default zeros).  ``out`` takes y (a [B, T, H] view; it must not overlap an input)."""
+    _sequence("z", z)
+    B, T, H = z.shape
+    _sequence("f", f, z)
+    if o is not None:
+        _sequence("o", o, z)
+    ctx = _context(ctx, z)
+    state = None if state is None else _rows("state", state, B, H, z.device)
+    with torch.cuda.device(z.device):
+        lens = _lengths(lens, B, T, z.device)
+        y = _output("out", out, z)
+        final = torch.empty((B, H), dtype=torch.float32, device=z.device)
+        states = torch.empty((B, (T + _lib.T2_SCAN_SPAN - 1) // _lib.T2_SCAN_SPAN, H), dtype=torch.float32, device=z.device) if tape else None
+        ws, n = _workspace(ctx, B, T, H)
+        args = _lib.T2ScanArgs(_DTYPES[z.dtype], B, T, H, int(bool(reverse)), _seq(z), _seq(f), _seq(o), _seq(y), _ptr(lens), _ptr(state),
+                               final.data_ptr(), _ptr(states), _seq(None), _seq(None), _seq(None), _seq(None), None, None, _ptr(ws), n)
+        with ctx.ordered():
+            _lib.check(ctx.lib.t2_gated_scan(ctx.handle, args))
+    return (y, final, ScanTape(z, f, o, lens, bool(reverse), states)) if tape else (y, final)
+
+
+def gated_scan_backward(ctx, tape: ScanTape, dy, dfinal=None):
+    """(dz, df, do, dstate): the gradients of the tape's inputs and of the state in front of the first step, for dy [B, T, H] (any
+    batch and time strides) and dfinal [B, H] (fp32, the gradient of the final state, default zeros).  ``do`` is None without an
+    output gate.  Positions behind a row's length get zeros.  An input that was broadcast gets the gradient of every place it went
+    to: sum it over that axis.  A tape serves any number of backward passes."""
+    z = tape.z
+    B, T, H = z.shape
+    _sequence("dy", dy, z)
+    ctx = _context(ctx, z)
+    dfinal = None if dfinal is None else _rows("dfinal", dfinal, B, H, z.device)
+    with torch.cuda.device(z.device):
+        dz, df = _output("dz", None, z), _output("df", None, z)
+        do = None if tape.o is None else _output("do", None, z)
+        dstate = torch.empty((B, H), dtype=torch.float32, device=z.device)
+        ws, n = _workspace(ctx, B, T, H)
+        args = _lib.T2ScanArgs(_DTYPES[z.dtype], B, T, H, int(tape.reverse), _seq(z), _seq(tape.f), _seq(tape.o), _seq(None), _ptr(tape.lens), None,
+                               None, tape.states.data_ptr(), _seq(dy), _seq(dz), _seq(df), _seq(do), _ptr(dfinal), dstate.data_ptr(), _ptr(ws), n)
+        with ctx.ordered():
+            _lib.check(ctx.lib.t2_gated_scan_backward(ctx.handle, args))
+    return dz, df, do, dstate
+
+
+def gated_scan_step(ctx, z, f, o, state, active=None, out=None):
+    """One new position for every row: z, f, o (or None) [B, H] -> y [B, H]; ``state`` [B, H] (fp32) is updated in place.  Rows where
+    ``active`` (bool [B] on the device) is False keep their state and get y = 0."""
+    for what, t in (("z", z), ("f", f), ("o", o), ("out", out)):
+        if t is None and what in ("o", "out"):
+            continue
+        if not (isinstance(t, torch.Tensor) and t.is_cuda) or t.dim() != 2 or t.dtype not in _DTYPES or 0 in t.shape:
+            raise ValueError(f"{what} must be a non-empty [B, H] device tensor of float32, bfloat16 or float16")
+        if t.shape != z.shape or t.dtype != z.dtype or t.device != z.device:
+            raise ValueError(f"{what} must be {z.dtype} {tuple(z.shape)} on {z.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+        if t.shape[1] > 1 and t.stride(1) != 1:
+            raise ValueError(f"the channels of {what} must be contiguous")
+    B, H = z.shape
+    if not (isinstance(state, torch.Tensor) and state.device == z.device and state.dtype == torch.float32 and state.shape == z.shape
+            and (H == 1 or state.stride(1) == 1)):
+        raise ValueError(f"state must be a float32 [{B}, {H}] tensor on {z.device} with contiguous rows")
+    if active is not None and not (isinstance(active, torch.Tensor) and active.device == z.device and active.dtype == torch.bool
+                                   and tuple(active.shape) == (B,)):
+        raise ValueError(f"active must be a bool [{B}] tensor on {z.device}")
+    ctx = _context(ctx, z)
+    with torch.cuda.device(z.device):
+        active = None if active is None else active.contiguous()
+        y = torch.empty((B, H), dtype=z.dtype, device=z.device) if out is None else out
+        with ctx.ordered():
+            _lib.check(ctx.lib.t2_gated_scan_step(ctx.handle, _DTYPES[z.dtype], B, H, z.data_ptr(), z.stride(0), f.data_ptr(), f.stride(0), _ptr(o),
+                                                  0 if o is None else o.stride(0), state.data_ptr(), state.stride(0), _ptr(active), y.data_ptr(),
+                                                  y.stride(0)))
+    return y

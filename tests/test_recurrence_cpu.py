@@ -1,0 +1,77 @@
+"""Refusals of the gated linear recurrence that need no GPU, and the 64-bit restatement's gradients against differences."""
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+
+from tacotron2_amd import _lib
+from tests import recurrence_ref as ref
+
+
+def _args(**kw):
+    a = _lib.T2ScanArgs()
+    a.dtype, a.B, a.T, a.H = 0, 2, 3, 4
+    for name in ("z", "f", "y", "dy", "dz", "df"):
+        setattr(a, name, (16, 12, 4))
+    a.tape = 16
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+def test_library_refuses_bad_arguments_before_any_device_work():
+    lib = _lib.load()
+    ctx = C.create_string_buffer(64)                 # never looked into: every call below is refused first
+    null = (None, 0, 0)
+    for fn, bad in ((lib.t2_gated_scan, [{"dtype": 3}, {"dtype": -1}, {"B": 0}, {"B": 65536}, {"T": 0}, {"T": (1 << 30) + 1}, {"H": 0}, {"H": (1 << 24) + 1},
+                                         {"z": null}, {"f": null}, {"y": null}]),
+                    (lib.t2_gated_scan_backward, [{"dy": null}, {"dz": null}, {"df": null}, {"o": (16, 12, 4)}, {"tape": None}, {"z": null}, {"dtype": 7}])):
+        assert fn(None, _args()) == _lib.T2_EINVAL and fn(ctx, None) == _lib.T2_EINVAL
+        for kw in bad:
+            assert fn(ctx, _args(**kw)) == _lib.T2_EINVAL, kw
+    step = lambda **kw: lib.t2_gated_scan_step(*{**dict(ctx=ctx, dtype=0, B=2, H=4, z=16, zs=4, f=16, fs=4, o=None, os=0, state=16, ss=4, active=None,  # noqa: E731
+                                                        y=16, ys=4), **kw}.values())
+    for kw in ({"ctx": None}, {"dtype": 5}, {"B": 0}, {"H": 0}, {"z": None}, {"f": None}, {"state": None}, {"y": None}, {"ss": 3}, {"ys": 3}):
+        assert step(**kw) == _lib.T2_EINVAL, kw
+    assert lib.t2_gated_scan_tape(2, 65, 3) == 2 * 2 * 3 and lib.t2_gated_scan_tape(0, 1, 1) < 0 and lib.t2_gated_scan_ws(1, 0, 1) < 0
+    big = lib.t2_gated_scan_tape(64, 1 << 30, 1 << 12)                               # counts beyond 32 bits
+    assert big == 64 * (1 << 24) * (1 << 12)
+
+
+def test_python_layer_refuses_host_tensors():
+    from tacotron2_amd import recurrence as R
+    z = torch.zeros(1, 2, 3)
+    with pytest.raises(ValueError):
+        R.gated_scan(None, z, z)
+    with pytest.raises(ValueError):
+        R.gated_scan_step(None, z[0], z[0], None, z[0])
+
+
+@pytest.mark.parametrize("reverse", [False, True])
+def test_restatement_against_a_loop_and_differences(reverse):
+    rng = np.random.default_rng(3)
+    z, f, o, dy = (rng.standard_normal((2, 6, 3)) for _ in range(4))
+    state, dfinal, lens = rng.standard_normal((2, 3)), rng.standard_normal((2, 3)), np.array([6, 4])
+
+    def loss(z, f, o, state):
+        total = 0.0
+        for b in range(2):
+            h = state[b].copy()
+            order = range(lens[b] - 1, -1, -1) if reverse else range(lens[b])
+            for t in order:
+                a = 1 / (1 + np.exp(-f[b, t]))
+                h = a * h + (1 - a) * z[b, t]
+                total += (dy[b, t] * h / (1 + np.exp(-o[b, t]))).sum()
+            total += (dfinal[b] * h).sum()
+        return total
+    x = ref.forward(z, f, o, lens, state, reverse)
+    assert abs((x["y"] * dy).sum() + (x["final"] * dfinal).sum() - loss(z, f, o, state)) < 1e-12
+    g = ref.backward(x, dy, dfinal, lens, reverse)
+    for i, k in enumerate(("dz", "df", "do", "dstate")):
+        base = [z, f, o, state]
+        for at in np.ndindex(base[i].shape):
+            up, down = [v.copy() for v in base], [v.copy() for v in base]
+            up[i][at] += 1e-5
+            down[i][at] -= 1e-5
+            assert abs((loss(*up) - loss(*down)) / 2e-5 - g[k][at]) < 1e-8
