@@ -13,7 +13,7 @@
  *  - "dev" pointers are HIP device pointers on the ctx's device (e.g. torch.Tensor.data_ptr());
  *    "host" pointers are ordinary host memory.  The caller owns every I/O buffer; the library owns
  *    weights and workspaces inside its handles.
- *  - all floating point is IEEE fp32; ids / lengths are int64 (util/tfrecord.py:108-109).
+ *  - all floating point is IEEE fp32 where an entry point names no other type; ids / lengths are int64 (util/tfrecord.py:108-109).
  *  - a handle is not thread-safe; use one ctx per GPU per thread.  All work is enqueued on the
  *    ctx's stream.  Host synchronisation: t2_decode_free() / t2_decode_free_finish() (to return
  *    steps_out); and every call that runs a persistent kernel (below) waits for it once, to read
@@ -471,6 +471,34 @@ int t2_gated_scan(t2_ctx* ctx, const t2_scan_args* a);
 int t2_gated_scan_backward(t2_ctx* ctx, const t2_scan_args* a);
 int t2_gated_scan_step(t2_ctx* ctx, int dtype, int B, int H, const void* z, int64_t z_stride, const void* f, int64_t f_stride, const void* o,
                        int64_t o_stride, float* state, int64_t state_stride, const uint8_t* active, void* y, int64_t y_stride);
+
+/* ---- AdamW over many tensors at once (beside t2_optim_*; the reference's optimizer is TF's Adam without decay) ---------------------
+ * One step of decoupled weight decay over n_tensors tensors of fp32, bf16 or fp16 (parameters and gradients each in a type of their own):
+ *     g' = gs g, gs = grad_scale * clip / max(grad_scale * |g|, clip) with the norm over all tensors (clip <= 0: gs = grad_scale)
+ *     m' = b1 m + (1 - b1) g'      v' = b2 v + (1 - b2) g'^2
+ *     p' = p (1 - lr decay) - lr / (1 - b1^t) * m' / (sqrt(v' / (1 - b2^t)) + epsilon)
+ * Arithmetic is fp32 (the norm and the factors of a step: double); p' is rounded once to the parameter's type and once to its copy's.
+ *  - States are the caller's buffers, kept alive with the handle: m, v dev [t2_adamw_elements()], 16-byte aligned; tensor i's start at the
+ *    sum of the sizes in front of it, each rounded up to 128.  state_bits 32: fp32.  state_bits 8: m and sqrt(v) as OCP e4m3 bytes, m_scale /
+ *    v_scale one e8m0 byte (2^(byte - 127), 255 = NaN) for every 128; codes are rounded stochastically by the counter-based generator
+ *    (csrc/rng.h) at (seed, stream 20, t, element), a root above zero never to zero.  A block that got a non-finite value stays NaN.
+ *  - step: dev int64, the number of steps taken; the device counts, so a captured step counts at every replay.
+ *  - t2_adamw_bind writes a table (dev, t2_adamw_table_bytes(), 16-byte aligned) of the tensors' addresses and types on the stream; the
+ *    other calls read it.  params may be NULL for a table that only serves the norm; copies (NULL, or NULL entries) get p' in their own type.
+ *  - learning_rate_dev: dev float that replaces learning_rate, or NULL.  skip_nonfinite: a step whose gradient norm is inf or NaN changes
+ *    nothing and is not counted.  Without it a NaN reaches the elements that have it (and their blocks of 128 in 8 bits).
+ * Calls for one handle must follow one another on the device; the handle's workspace belongs to the call that runs. */
+typedef struct t2_adamw t2_adamw;
+int64_t t2_adamw_elements(int n_tensors, const int64_t* sizes);
+int t2_adamw_create(t2_ctx* ctx, int n_tensors, const int64_t* sizes, const double* decay, double beta1, double beta2, double epsilon, int state_bits,
+                    uint32_t seed, void* m, void* v, void* m_scale, void* v_scale, int64_t* step, t2_adamw** out);
+int t2_adamw_destroy(t2_adamw* o);
+int64_t t2_adamw_table_bytes(const t2_adamw* o);
+int t2_adamw_bind(t2_ctx* ctx, t2_adamw* o, const void* const* grads, const int32_t* grad_types, void* const* params, const int32_t* param_types,
+                  void* const* copies, const int32_t* copy_types, void* table);
+int t2_adamw_global_norm(t2_ctx* ctx, t2_adamw* o, const void* table, double grad_scale, float* norm_out /* dev [1] */);
+int t2_adamw_step(t2_ctx* ctx, t2_adamw* o, const void* table, double learning_rate, const float* learning_rate_dev, double clip_norm, double grad_scale,
+                  int skip_nonfinite);
 
 #ifdef __cplusplus
 }

@@ -157,6 +157,14 @@ _SIGS.update({
     "t2_gated_scan": (C.c_int, [_p, C.POINTER(T2ScanArgs)]),
     "t2_gated_scan_backward": (C.c_int, [_p, C.POINTER(T2ScanArgs)]),
     "t2_gated_scan_step": (C.c_int, [_p, C.c_int, C.c_int, C.c_int, _p, C.c_int64, _p, C.c_int64, _p, C.c_int64, _p, C.c_int64, _p, _p, C.c_int64]),
+    "t2_adamw_elements": (C.c_int64, [C.c_int, _i64p]),
+    "t2_adamw_create": (C.c_int, [_p, C.c_int, _i64p, C.POINTER(C.c_double), C.c_double, C.c_double, C.c_double, C.c_int, C.c_uint32, _p, _p, _p, _p, _p,
+                                  C.POINTER(_p)]),
+    "t2_adamw_destroy": (C.c_int, [_p]),
+    "t2_adamw_table_bytes": (C.c_int64, [_p]),
+    "t2_adamw_bind": (C.c_int, [_p, _p, C.POINTER(_p), C.POINTER(C.c_int32), C.POINTER(_p), C.POINTER(C.c_int32), C.POINTER(_p), C.POINTER(C.c_int32), _p]),
+    "t2_adamw_global_norm": (C.c_int, [_p, _p, _p, C.c_double, _p]),
+    "t2_adamw_step": (C.c_int, [_p, _p, _p, C.c_double, _p, C.c_double, C.c_double, C.c_int]),
 })
 
 _lib = None

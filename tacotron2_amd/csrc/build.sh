@@ -6,7 +6,7 @@ cd "$(dirname "$0")"
 HIPCC=${HIPCC:-/opt/rocm/bin/hipcc}
 FLAGS=(--offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wall -Wno-unused-function -Wno-unused-value
        -Xclang -target-feature -Xclang -packed-fp32-ops)
-UNITS=(t2mi recurrence)
+UNITS=(t2mi recurrence adamw)
 mkdir -p build
 pids=()
 for u in "${UNITS[@]}"; do

@@ -18,7 +18,9 @@ import numpy as np
 import torch
 
 from . import _lib
-from .engine import Context
+from .engine import Context, stream_context
+
+_TYPES = {torch.float32: _lib.T2_F32, torch.bfloat16: _lib.T2_BF16, torch.float16: _lib.T2_F16}
 
 
 def _ctx_of(obj) -> Context:
@@ -255,6 +257,182 @@ class AdamOptimizer:
     def close(self):
         if getattr(self, "_h", None) and getattr(self.ctx, "handle", None):
             self.ctx.lib.t2_optim_destroy(self._h)
+        self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class AdamWBinding:
+    """The tensors of a step, checked once, and their table on the device (``AdamW.bind``).  It stays valid as long as it is kept;
+    it keeps the tensors."""
+
+    def __init__(self, table, grads, params, copies):
+        self.table, self.grads, self.params, self.copies = table, grads, params, copies
+
+
+class AdamW:
+    """Adam with decoupled weight decay over many tensors at once, fused with clipping by the norm of all gradients.
+
+    ``sizes``: the number of elements of every tensor (or one number), or a ``flatten_spec``: the tensors are then the variables of one flat
+    buffer, gradients and parameters may be given as that buffer, and a single ``weight_decay`` applies to the variables of two
+    dimensions and more (kernels; not biases, norms and moving statistics).  ``weight_decay``: one factor, or one for every tensor.
+    Parameters and gradients are fp32, bf16 or fp16, each tensor in a type of its own; ``copies`` (with fp32 parameters: the tensors that
+    the next forward pass reads) get the new values in their type in the same pass.  ``state_bits=32``: fp32 moments.  ``state_bits=8``:
+    ``m`` and the root of ``v`` as float8_e4m3fn with one power of two (float8_e8m0fnu) for 128 elements, rounded stochastically by
+    (``seed``, step, element): 2 bytes an element in place of 8.  The difference from AdamOptimizer's TF form: bias corrections on both
+    moments, epsilon beside the corrected root, weight decay.
+
+    ``m``, ``v``, ``m_scale``, ``v_scale`` are the live states, tensor i's from ``offsets[i]`` on (``load_state`` sets them).  The step count is
+    on the device (``steps()``), so a captured step counts at every replay; capture with a learning rate that is a device scalar
+    where it changes.  ``ctx``: a Context, an Engine, or None for torch's current stream; creating one synchronises, a step does not.
+    Trainer.train_step takes an AdamW of its ``flatten_spec`` in AdamOptimizer's place."""
+
+    def __init__(self, ctx, sizes, learning_rate=0.001, beta1=0.9, beta2=0.999, epsilon=1e-8, weight_decay=0.01, state_bits=32, seed=0, device=None):
+        self._ctx = None if ctx is None else _ctx_of(ctx)
+        own = self._ctx or stream_context(device)
+        self.device = own.device
+        sizes = list(sizes) if isinstance(sizes, (list, tuple)) else [sizes]
+        self.spec = None
+        if sizes and isinstance(sizes[0], (list, tuple)):
+            self.spec, sizes = sizes, [size for _, _, _, size in sizes]
+            if not isinstance(weight_decay, (list, tuple)):
+                weight_decay = [weight_decay if len(shape) >= 2 else 0.0 for _, shape, _, _ in self.spec]
+        self.sizes = [int(n) for n in sizes]
+        decay = [float(w) for w in weight_decay] if isinstance(weight_decay, (list, tuple)) else [float(weight_decay)] * len(self.sizes)
+        if len(decay) != len(self.sizes):
+            raise ValueError(f"{len(decay)} weight decays for {len(self.sizes)} tensors")
+        self.learning_rate, self.state_bits, self.seed = learning_rate, int(state_bits), int(seed) & 0xFFFFFFFF
+        self._h = C.c_void_p()
+        k = len(self.sizes)
+        csizes = (C.c_int64 * max(k, 1))(*self.sizes)
+        lib = self._lib = own.lib
+        total = lib.t2_adamw_elements(k, csizes)
+        if total < 0:
+            _lib.check(int(total))
+        self.offsets, at = [], 0
+        for n in self.sizes:
+            self.offsets.append(at)
+            at += (n + 127) // 128 * 128
+        with torch.cuda.device(self.device):
+            small = self.state_bits == 8
+            new = lambda n, dt: torch.zeros(n, dtype=torch.uint8 if dt.itemsize == 1 else dt, device=self.device).view(dt)  # noqa: E731
+            self.m, self.v = (new(total, torch.float8_e4m3fn if small else torch.float32) for _ in range(2))
+            self.m_scale, self.v_scale = (new(total // 128, torch.float8_e8m0fnu) for _ in range(2)) if small else (None, None)
+            self._step = torch.zeros(1, dtype=torch.int64, device=self.device)
+            scales = [None if t is None else t.data_ptr() for t in (self.m_scale, self.v_scale)]
+            _lib.check(lib.t2_adamw_create(own.handle, k, csizes, (C.c_double * k)(*decay), float(beta1), float(beta2), float(epsilon), self.state_bits,
+                                           self.seed, self.m.data_ptr(), self.v.data_ptr(), *scales, self._step.data_ptr(), C.byref(self._h)))
+
+    def _context(self):
+        return self._ctx or stream_context(self.device.index)
+
+    def _tensors(self, what, ts, optional=False):
+        if isinstance(ts, torch.Tensor) and self.spec is not None:
+            if ts.dim() != 1 or not ts.is_contiguous() or ts.numel() < flat_size(self.spec):
+                raise ValueError(f"{what} must be a contiguous flat buffer of {flat_size(self.spec)} elements")
+            ts = [ts[off:off + size] for _, _, off, size in self.spec]
+        ts = [ts] if isinstance(ts, torch.Tensor) else list(ts)
+        if len(ts) != len(self.sizes):
+            raise ValueError(f"{len(ts)} {what} for {len(self.sizes)} tensors")
+        for i, (t, n) in enumerate(zip(ts, self.sizes)):
+            if t is None and optional:
+                continue
+            if not (isinstance(t, torch.Tensor) and t.device == self.device and t.dtype in _TYPES and t.is_contiguous() and t.numel() == n):
+                raise ValueError(f"{what}[{i}] must be a contiguous float32, bfloat16 or float16 tensor of {n} elements on {self.device}")
+        return ts
+
+    def bind(self, grads, params=None, copies=None) -> AdamWBinding:
+        """Check the tensors of the steps to come and write their table (stream-ordered, nothing synchronises).  Gradients are only
+        read; no parameter or copy may overlap another tensor of the step.  Without ``params`` the binding serves ``global_norm`` alone."""
+        grads = self._tensors("grads", grads)
+        params = None if params is None else self._tensors("params", params)
+        copies = None if copies is None else self._tensors("copies", copies, optional=True)
+        if copies is not None and params is None:
+            raise ValueError("copies need params")
+        spans = [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), w) for ts, w in ((grads, False), (params, True), (copies, True))
+                 for t in ts or () if t is not None]
+        read_to = written_to = 0
+        for first, end, written in sorted(spans):
+            if first < written_to or (written and first < read_to):
+                raise ValueError("a parameter or copy overlaps another tensor")
+            read_to, written_to = max(read_to, end), max(written_to, end if written else 0)
+        k = len(self.sizes)
+
+        def column(ts):
+            if ts is None:
+                return None, None
+            return (C.c_void_p * k)(*[None if t is None else t.data_ptr() for t in ts]), (C.c_int32 * k)(*[0 if t is None else _TYPES[t.dtype] for t in ts])
+        ctx = self._context()
+        with torch.cuda.device(self.device):
+            table = torch.empty(self._lib.t2_adamw_table_bytes(self._h), dtype=torch.uint8, device=self.device)
+            with ctx.ordered():
+                _lib.check(self._lib.t2_adamw_bind(ctx.handle, self._h, *column(grads), *column(params), *column(copies), table.data_ptr()))
+        return AdamWBinding(table, grads, params, copies)
+
+    def global_norm(self, grads, grad_scale: float = 1.0) -> torch.Tensor:
+        """The norm of grad_scale * all gradients (dev scalar)."""
+        b = grads if isinstance(grads, AdamWBinding) else self.bind(grads)
+        ctx = self._context()
+        with torch.cuda.device(self.device):
+            out = torch.empty(1, dtype=torch.float32, device=self.device)
+            with ctx.ordered():
+                _lib.check(self._lib.t2_adamw_global_norm(ctx.handle, self._h, b.table.data_ptr(), float(grad_scale), out.data_ptr()))
+        return out[0]
+
+    def apply_gradients(self, grads, params=None, global_step: int = 0, clip_norm: float = 1.0, grad_scale: float = 1.0, copies=None,
+                        skip_nonfinite: bool = False) -> int:
+        """One step on ``params`` in place (``grads``: tensors, or an AdamWBinding of gradients and parameters); returns global_step + 1.
+        ``clip_norm <= 0`` does not clip.  ``skip_nonfinite``: gradients whose norm is inf or NaN change nothing (``steps()`` stays)."""
+        if isinstance(grads, AdamWBinding):
+            b = grads
+            if params is not None or copies is not None:
+                raise ValueError("a binding has its own params and copies")
+        else:
+            if params is None:
+                raise ValueError("params are needed")
+            b = self.bind(grads, params, copies)
+        if b.params is None:
+            raise ValueError("this binding has no params")
+        lr = self.learning_rate(global_step) if callable(self.learning_rate) else self.learning_rate
+        lr_dev = None
+        if isinstance(lr, torch.Tensor):
+            if not (lr.device == self.device and lr.dtype == torch.float32 and lr.numel() == 1):
+                raise ValueError(f"a learning rate on the device must be one float32 on {self.device}")
+            lr_dev, lr = lr.data_ptr(), 0.0
+        ctx = self._context()
+        with torch.cuda.device(self.device), ctx.ordered():
+            _lib.check(self._lib.t2_adamw_step(ctx.handle, self._h, b.table.data_ptr(), float(lr), lr_dev, float(clip_norm), float(grad_scale),
+                                               int(bool(skip_nonfinite))))
+        return global_step + 1
+
+    def steps(self) -> int:
+        """The number of steps taken (synchronises)."""
+        return int(self._step)
+
+    def state(self):
+        """(m, v, steps, m_scale, v_scale): copies of the states, as ``load_state`` takes them."""
+        return tuple(None if t is None else t.clone() for t in (self.m, self.v)) + (self.steps(),) + \
+            tuple(None if t is None else t.clone() for t in (self.m_scale, self.v_scale))
+
+    def load_state(self, m, v, step: int, m_scale=None, v_scale=None):
+        if step < 0:
+            raise ValueError("the step count cannot be negative")
+        for what, src, dst in (("m", m, self.m), ("v", v, self.v), ("m_scale", m_scale, self.m_scale), ("v_scale", v_scale, self.v_scale)):
+            if (src is None) != (dst is None) or (dst is not None and (src.dtype != dst.dtype or src.shape != dst.shape)):
+                raise ValueError(f"{what} must be {'None' if dst is None else f'{dst.dtype} {tuple(dst.shape)}'}")
+        for src, dst in ((m, self.m), (v, self.v), (m_scale, self.m_scale), (v_scale, self.v_scale)):
+            if dst is not None:
+                raw = torch.uint8 if dst.dtype.itemsize == 1 else dst.dtype
+                dst.view(raw).copy_(src.view(raw))
+        self._step.fill_(int(step))
+
+    def close(self):
+        if getattr(self, "_h", None):
+            self._lib.t2_adamw_destroy(self._h)
         self._h = None
 
     def __del__(self):

@@ -6,5 +6,5 @@ cd "$(dirname "$0")/.."
 mkdir -p tools/bin
 /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -shared -Wno-unused-function -Wno-unused-value \
     -Xclang -target-feature -Xclang -packed-fp32-ops -DPZ_NO_WEIGHT_STREAM \
-    -o tools/bin/libt2mi_noweights.so tacotron2_amd/csrc/{t2mi,recurrence}.hip
+    -o tools/bin/libt2mi_noweights.so tacotron2_amd/csrc/{t2mi,recurrence,adamw}.hip
 echo built tools/bin/libt2mi_noweights.so
