@@ -9,8 +9,7 @@
 // memory of n steps collects n of them (800 steps, memories up to 1000: the final state was off by 1.5e-6, now by what the
 // rounding of a itself leaves).  exp2 of more than 126 would overflow and make b inf * 0; NaN passes through.
 __device__ __forceinline__ void gate(float f, float& a, float& b) {
-    float x = -SCAN_LOG2E * f;
-    x = x > 126.f ? 126.f : x;
+    const float x = __builtin_elementwise_minimum(-SCAN_LOG2E * f, 126.f);
     const float e = __builtin_amdgcn_exp2f(x), d = 1.f + e, r = __builtin_amdgcn_rcpf(d);
     a = fmaf(fmaf(-d, r, 1.f), r, r);
     b = e * a;
@@ -166,7 +165,17 @@ __global__ __launch_bounds__(16 * TG) void scan_tile_kernel(t2_scan_args a, Scan
             float b;
             gate(E::at(fr[l], j), ga[l][j], b);
             x[l][j] = b * E::at(zr[l], j);
-            if (s0 + l >= len) { ga[l][j] = 1.f; x[l][j] = 0.f; }
+        }
+    if (s0 + L > len) {                                      // padding: h stays
+#pragma unroll
+        for (int l = 0; l < L; ++l)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) if (s0 + l >= len) { ga[l][j] = 1.f; x[l][j] = 0.f; }
+    }
+#pragma unroll
+    for (int l = 0; l < L; ++l)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
             B[j] = fmaf(ga[l][j], B[j], x[l][j]);
             A[j] *= ga[l][j];
         }
@@ -377,15 +386,9 @@ extern "C" int64_t t2_gated_scan_tape(int B, int T, int H) {
     return (int64_t)B * ((T + T2_SCAN_SPAN - 1) / T2_SCAN_SPAN) * H;
 }
 
-// steps of a tile
-#ifndef SCAN_FWD_TG
-#define SCAN_FWD_TG 16
-#define SCAN_FWD_L 8
-#endif
-#ifndef SCAN_BWD_TG
-#define SCAN_BWD_TG 16
-#define SCAN_BWD_L 4
-#endif
+// Steps of a tile (16 lanes x TG threads of L steps)
+template <bool BACKWARD> static int tile_steps(int T) { return BACKWARD ? (T <= 64 ? 64 : T <= 256 ? 256 : 64) : (T <= 64 ? 64 : 256); }
+
 static int64_t ws_bytes(int B, int T, int H, int steps) {
     const int64_t ntile = (T + steps - 1) / steps, chains = (int64_t)B * ((H + SCAN_CH - 1) / SCAN_CH);
     if (ntile * chains > 0x7FFFFFFF) return fail(T2_EINVAL, "[%d,%d,%d] is too large for one call", B, T, H);
@@ -394,7 +397,7 @@ static int64_t ws_bytes(int B, int T, int H, int steps) {
 
 extern "C" int64_t t2_gated_scan_ws(int B, int T, int H) {
     if (!sizes_ok(B, T, H)) return fail(T2_EINVAL, "bad shape [%d,%d,%d]", B, T, H);
-    const int64_t f = ws_bytes(B, T, H, SCAN_FWD_TG * SCAN_FWD_L), g = ws_bytes(B, T, H, SCAN_BWD_TG * SCAN_BWD_L);
+    const int64_t f = ws_bytes(B, T, H, tile_steps<false>(T)), g = ws_bytes(B, T, H, tile_steps<true>(T));
     return f < 0 || g < 0 ? T2_EINVAL : f > g ? f : g;
 }
 
@@ -421,22 +424,27 @@ static bool vectors(const t2_scan_args* a, const t2_seq* const* q, int n) {
     return true;
 }
 
-template <typename E, bool GATE, bool VEC, bool BACKWARD>
-static int launch(t2_ctx* ctx, const t2_scan_args* a) {
-    constexpr int TG = BACKWARD ? SCAN_BWD_TG : SCAN_FWD_TG, L = BACKWARD ? SCAN_BWD_L : SCAN_FWD_L;
+template <typename E, bool GATE, bool VEC, bool BACKWARD, int TG, int L>
+static int launch_tiles(t2_ctx* ctx, const t2_scan_args* a) {
     const int ntile = (a->T + TG * L - 1) / (TG * L);
     const int64_t blocks = (int64_t)ntile * a->B * ((a->H + SCAN_CH - 1) / SCAN_CH);
     ScanWs w = {};
     if (ntile > 1) {
         w = scan_ws(a->ws, blocks * SCAN_CH);
-        const long long n16 = ws_bytes(a->B, a->T, a->H, TG * L) / 16;
-        const long long nb = (n16 + 1023) / 1024;
+        const long long n16 = ws_bytes(a->B, a->T, a->H, TG * L) / 16, nb = (n16 + 1023) / 1024;
         hipLaunchKernelGGL(scan_ws_kernel, dim3((unsigned)(nb < 2048 ? nb : 2048)), dim3(256), 0, ctx->stream, (uint4*)a->ws, n16);
     }
     if constexpr (BACKWARD) hipLaunchKernelGGL((scan_tile_backward_kernel<E, GATE, VEC, TG, L>), dim3((unsigned)blocks), dim3(16 * TG), 0, ctx->stream, *a, w, ntile);
     else hipLaunchKernelGGL((scan_tile_kernel<E, GATE, VEC, TG, L>), dim3((unsigned)blocks), dim3(16 * TG), 0, ctx->stream, *a, w, ntile);
     HIP_TRY(hipGetLastError());
     return T2_OK;
+}
+
+template <typename E, bool GATE, bool VEC, bool BACKWARD>
+static int launch(t2_ctx* ctx, const t2_scan_args* a) {
+    const int steps = tile_steps<BACKWARD>(a->T);
+    if constexpr (BACKWARD) return steps == 64 ? launch_tiles<E, GATE, VEC, true, 16, 4>(ctx, a) : launch_tiles<E, GATE, VEC, true, 64, 4>(ctx, a);
+    else return steps == 64 ? launch_tiles<E, GATE, VEC, false, 8, 8>(ctx, a) : launch_tiles<E, GATE, VEC, false, 32, 8>(ctx, a);
 }
 
 template <bool BACKWARD>

@@ -137,6 +137,17 @@ def shared_context(device: int = 0) -> Context:
     return _shared[device]
 
 
+class _Nothing:
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_NOTHING = _Nothing()
+
+
 class StreamContext(Context):
     """A context on a stream of the caller's: the library enqueues where the caller's other work is, and ``ordered`` has nothing
     to order.  Creating one leaves torch's current device as it was."""
@@ -149,9 +160,8 @@ class StreamContext(Context):
         with torch.cuda.device(self.device):
             _lib.check(self.lib.t2_ctx_create_on_stream(device, C.c_void_p(stream.cuda_stream), C.byref(self.handle)))
 
-    @contextlib.contextmanager
     def ordered(self):
-        yield
+        return _NOTHING
 
 
 _on_stream: Dict[tuple, StreamContext] = {}
@@ -160,15 +170,16 @@ _on_stream: Dict[tuple, StreamContext] = {}
 def stream_context(device: Optional[int] = None) -> StreamContext:
     """The context of torch's current stream on ``device`` (default: the current device).  It holds no workspace, so it serves
     the entry points that take theirs from the caller (recurrence, AdamW)."""
-    if not torch.cuda.is_available():
-        raise RuntimeError("tacotron2_amd needs an MI355X (gfx950) GPU: there is no CPU path")
     if device is None:
+        if not torch.cuda.is_available():
+            raise RuntimeError("tacotron2_amd needs an MI355X (gfx950) GPU: there is no CPU path")
         device = torch.cuda.current_device()
-    stream = torch.cuda.current_stream(device)
-    key = (device, stream.cuda_stream, threading.get_ident())
-    if key not in _on_stream:
-        _on_stream[key] = StreamContext(device, stream)
-    return _on_stream[key]
+    # the bare handle: torch.cuda.current_stream() builds an object, 2 us of a call's 10
+    key = (device, torch._C._cuda_getCurrentRawStream(device), threading.get_ident())
+    ctx = _on_stream.get(key)
+    if ctx is None:
+        ctx = _on_stream[key] = StreamContext(device, torch.cuda.current_stream(device))
+    return ctx
 
 
 class Engine:

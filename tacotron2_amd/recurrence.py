@@ -34,7 +34,7 @@ class ScanTape(NamedTuple):
 
 def _context(ctx, t: torch.Tensor) -> Context:
     if ctx is None:
-        return stream_context(t.device.index)
+        return stream_context(t.get_device())
     ctx = ctx if isinstance(ctx, Context) else ctx.context
     if ctx.device != t.device:
         raise ValueError(f"tensors on {t.device}, context on {ctx.device}")
@@ -86,15 +86,19 @@ def _lengths(lens, B: int, T: int, device) -> Optional[torch.Tensor]:
     return torch.from_numpy(host.astype(np.int64)).to(device)
 
 
+_NONE = (0, 0, 0)
+
+
 def _seq(t: Optional[torch.Tensor]):
-    return (None, 0, 0) if t is None else (t.data_ptr(), t.stride(0), t.stride(1))
+    return _NONE if t is None else (t.data_ptr(), *t.stride()[:2])
 
 
 def _ptr(t: Optional[torch.Tensor]):
-    return None if t is None else t.data_ptr()
+    return 0 if t is None else t.data_ptr()
 
 
 def _workspace(ctx: Context, B: int, T: int, H: int) -> Tuple[Optional[torch.Tensor], int]:
+    # a tensor of the call's own: a captured call's workspace is its graph's
     n = ctx.lib.t2_gated_scan_ws(B, T, H)
     if n < 0:
         _lib.check(_lib.T2_EINVAL)
@@ -115,17 +119,18 @@ def gated_scan(ctx, z, f, o=None, lens=None, state=None, reverse: bool = False, 
     if o is not None:
         _sequence("o", o, z)
     ctx = _context(ctx, z)
-    state = None if state is None else _rows("state", state, B, H, z.device)
-    with torch.cuda.device(z.device):
-        lens = _lengths(lens, B, T, z.device)
-        y = _output("out", out, z)
-        final = torch.empty((B, H), dtype=torch.float32, device=z.device)
-        states = torch.empty((B, (T + _lib.T2_SCAN_SPAN - 1) // _lib.T2_SCAN_SPAN, H), dtype=torch.float32, device=z.device) if tape else None
-        ws, n = _workspace(ctx, B, T, H)
-        args = _lib.T2ScanArgs(_DTYPES[z.dtype], B, T, H, int(bool(reverse)), _seq(z), _seq(f), _seq(o), _seq(y), _ptr(lens), _ptr(state),
-                               final.data_ptr(), _ptr(states), _seq(None), _seq(None), _seq(None), _seq(None), None, None, _ptr(ws), n)
-        with ctx.ordered():
-            _lib.check(ctx.lib.t2_gated_scan(ctx.handle, args))
+    device = z.device
+    if state is not None:
+        state = _rows("state", state, B, H, device)
+    lens = _lengths(lens, B, T, device)
+    y = _output("out", out, z)
+    final = torch.empty((B, H), dtype=torch.float32, device=device)
+    states = torch.empty((B, -(-T // _lib.T2_SCAN_SPAN), H), dtype=torch.float32, device=device) if tape else None
+    ws, n = _workspace(ctx, B, T, H)
+    args = _lib.T2ScanArgs.from_buffer_copy(_lib.SCAN_ARGS.pack(_DTYPES[z.dtype], B, T, H, 1 if reverse else 0, *_seq(z), *_seq(f), *_seq(o), *_seq(y), _ptr(lens), _ptr(state),
+                               final.data_ptr(), _ptr(states), *_NONE, *_NONE, *_NONE, *_NONE, 0, 0, _ptr(ws), n))
+    with ctx.ordered():
+        _lib.check(ctx.lib.t2_gated_scan(ctx.handle, args))
     return (y, final, ScanTape(z, f, o, lens, bool(reverse), states)) if tape else (y, final)
 
 
@@ -138,44 +143,43 @@ def gated_scan_backward(ctx, tape: ScanTape, dy, dfinal=None):
     B, T, H = z.shape
     _sequence("dy", dy, z)
     ctx = _context(ctx, z)
-    dfinal = None if dfinal is None else _rows("dfinal", dfinal, B, H, z.device)
-    with torch.cuda.device(z.device):
-        dz, df = _output("dz", None, z), _output("df", None, z)
-        do = None if tape.o is None else _output("do", None, z)
-        dstate = torch.empty((B, H), dtype=torch.float32, device=z.device)
-        ws, n = _workspace(ctx, B, T, H)
-        args = _lib.T2ScanArgs(_DTYPES[z.dtype], B, T, H, int(tape.reverse), _seq(z), _seq(tape.f), _seq(tape.o), _seq(None), _ptr(tape.lens), None,
-                               None, tape.states.data_ptr(), _seq(dy), _seq(dz), _seq(df), _seq(do), _ptr(dfinal), dstate.data_ptr(), _ptr(ws), n)
-        with ctx.ordered():
-            _lib.check(ctx.lib.t2_gated_scan_backward(ctx.handle, args))
+    device = z.device
+    if dfinal is not None:
+        dfinal = _rows("dfinal", dfinal, B, H, device)
+    dz, df = (torch.empty(z.shape, dtype=z.dtype, device=device) for _ in range(2))
+    do = None if tape.o is None else torch.empty(z.shape, dtype=z.dtype, device=device)
+    dstate = torch.empty((B, H), dtype=torch.float32, device=device)
+    ws, n = _workspace(ctx, B, T, H)
+    args = _lib.T2ScanArgs.from_buffer_copy(_lib.SCAN_ARGS.pack(_DTYPES[z.dtype], B, T, H, int(tape.reverse), *_seq(z), *_seq(tape.f), *_seq(tape.o), *_NONE, _ptr(tape.lens), 0, 0,
+                               tape.states.data_ptr(), *_seq(dy), *_seq(dz), *_seq(df), *_seq(do), _ptr(dfinal), dstate.data_ptr(), _ptr(ws), n))
+    with ctx.ordered():
+        _lib.check(ctx.lib.t2_gated_scan_backward(ctx.handle, args))
     return dz, df, do, dstate
 
 
 def gated_scan_step(ctx, z, f, o, state, active=None, out=None):
     """One new position for every row: z, f, o (or None) [B, H] -> y [B, H]; ``state`` [B, H] (fp32) is updated in place.  Rows where
     ``active`` (bool [B] on the device) is False keep their state and get y = 0."""
+    if not (isinstance(z, torch.Tensor) and z.is_cuda and z.dim() == 2 and z.dtype in _DTYPES and z.numel()):
+        raise ValueError("z must be a non-empty [B, H] device tensor of float32, bfloat16 or float16")
+    B, H = shape = z.shape
+    dtype, device = z.dtype, z.device
     for what, t in (("z", z), ("f", f), ("o", o), ("out", out)):
-        if t is None and what in ("o", "out"):
+        if t is None and (what == "o" or what == "out"):
             continue
-        if not (isinstance(t, torch.Tensor) and t.is_cuda) or t.dim() != 2 or t.dtype not in _DTYPES or 0 in t.shape:
-            raise ValueError(f"{what} must be a non-empty [B, H] device tensor of float32, bfloat16 or float16")
-        if t.shape != z.shape or t.dtype != z.dtype or t.device != z.device:
-            raise ValueError(f"{what} must be {z.dtype} {tuple(z.shape)} on {z.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
-        if t.shape[1] > 1 and t.stride(1) != 1:
-            raise ValueError(f"the channels of {what} must be contiguous")
-    B, H = z.shape
-    if not (isinstance(state, torch.Tensor) and state.device == z.device and state.dtype == torch.float32 and state.shape == z.shape
+        if not isinstance(t, torch.Tensor) or t.shape != shape or t.dtype != dtype or t.device != device or (H > 1 and t.stride(1) != 1):
+            raise ValueError(f"{what} must be a {dtype} {tuple(shape)} tensor on {device} with contiguous rows")
+    if not (isinstance(state, torch.Tensor) and state.device == device and state.dtype == torch.float32 and state.shape == shape
             and (H == 1 or state.stride(1) == 1)):
-        raise ValueError(f"state must be a float32 [{B}, {H}] tensor on {z.device} with contiguous rows")
-    if active is not None and not (isinstance(active, torch.Tensor) and active.device == z.device and active.dtype == torch.bool
-                                   and tuple(active.shape) == (B,)):
-        raise ValueError(f"active must be a bool [{B}] tensor on {z.device}")
+        raise ValueError(f"state must be a float32 [{B}, {H}] tensor on {device} with contiguous rows")
+    if active is not None:
+        if not (isinstance(active, torch.Tensor) and active.device == device and active.dtype == torch.bool and active.shape == shape[:1]):
+            raise ValueError(f"active must be a bool [{B}] tensor on {device}")
+        active = active.contiguous()
     ctx = _context(ctx, z)
-    with torch.cuda.device(z.device):
-        active = None if active is None else active.contiguous()
-        y = torch.empty((B, H), dtype=z.dtype, device=z.device) if out is None else out
-        with ctx.ordered():
-            _lib.check(ctx.lib.t2_gated_scan_step(ctx.handle, _DTYPES[z.dtype], B, H, z.data_ptr(), z.stride(0), f.data_ptr(), f.stride(0), _ptr(o),
-                                                  0 if o is None else o.stride(0), state.data_ptr(), state.stride(0), _ptr(active), y.data_ptr(),
-                                                  y.stride(0)))
+    y = torch.empty(shape, dtype=dtype, device=device) if out is None else out
+    with ctx.ordered():
+        _lib.check(ctx.lib.t2_gated_scan_step(ctx.handle, _DTYPES[dtype], B, H, z.data_ptr(), z.stride(0), f.data_ptr(), f.stride(0), _ptr(o),
+                                              0 if o is None else o.stride(0), state.data_ptr(), state.stride(0), _ptr(active), y.data_ptr(),
+                                              y.stride(0)))
     return y

@@ -404,7 +404,7 @@ class AdamW:
                 raise ValueError(f"a learning rate on the device must be one float32 on {self.device}")
             lr_dev, lr = lr.data_ptr(), 0.0
         ctx = self._context()
-        with torch.cuda.device(self.device), ctx.ordered():
+        with ctx.ordered():
             _lib.check(self._lib.t2_adamw_step(ctx.handle, self._h, b.table.data_ptr(), float(lr), lr_dev, float(clip_norm), float(grad_scale),
                                                int(bool(skip_nonfinite))))
         return global_step + 1
