@@ -33,30 +33,36 @@ __device__ __forceinline__ int row_length(const int64_t* lens, int b, int T) {
 // through the compositions in between in their order; the first tile of a group finds it through the whole group before and
 // publishes it.  The order of every sum is fixed, so results do not depend on timing, and only one hand-over in SCAN_GROUP
 // has to wait for another.  Every word is a value that carries its own validity (all ones: not there yet; a computed NaN is never
-// that pattern), so one relaxed agent-scope access hands it over, without flags or fences.  Tiles are numbered by a counter that
-// workgroups draw from as they start, all tiles of a step range before those that follow it: a workgroup waits only for workgroups
-// that have started before it and that wait for none behind them, so every wait ends.
+// that pattern), so one relaxed agent-scope access hands it over, without flags or fences.  A workgroup's chain (row and channels) is
+// its index's, its tile is drawn from the chain's counter as it starts: it waits only for workgroups of the chain that have started
+// before it and that wait for none behind them, so every wait ends.  (One counter for all chains: B=2, T=65536, H=1024 draws 8192
+// times from one address; every chain has a counter on a line of its own.)
 // ------------------------------------------------------------------------------------------------
-#define SCAN_CH 64
-#define SCAN_GROUP 16
+#ifndef SCAN_GROUP
+#define SCAN_GROUP 8
+#endif
+#ifndef SCAN_FW
+#define SCAN_FW 4
+#define SCAN_BW 3
+#endif
 #define SCAN_WAIT_TICKS 200000000ull   /* 2 s of the 100 MHz clock; a wait never comes near it.  Beyond: NaN, not a hang */
 
-struct ScanWs {                        // counter | compositions [ntile][chains][64] | states in front of the groups [ngroup][chains][64]
+struct ScanWs {                        // counters [chains][16] | compositions [ntile][chains][64] | states in front of the groups [ngroup][chains][64]
     unsigned* next;
     unsigned long long* piece;
     unsigned* state;
 };
-static __host__ __device__ inline ScanWs scan_ws(void* p, long long slots) {
+static inline ScanWs scan_ws(void* p, long long chains, long long slots) {
     ScanWs w;
     w.next = (unsigned*)p;
-    w.piece = (unsigned long long*)((char*)p + 16);
+    w.piece = (unsigned long long*)((char*)p + chains * 64);
     w.state = (unsigned*)(w.piece + slots);
     return w;
 }
 
-__global__ __launch_bounds__(256) void scan_ws_kernel(uint4* ws, long long n16) {
+__global__ __launch_bounds__(256) void scan_ws_kernel(uint4* ws, long long zeros, long long n16) {
     const uint4 ones = {~0u, ~0u, ~0u, ~0u}, zero = {0u, 0u, 0u, 0u};
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n16; i += (long long)gridDim.x * 256) ws[i] = i == 0 ? zero : ones;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n16; i += (long long)gridDim.x * 256) ws[i] = i < zeros ? zero : ones;
 }
 
 __device__ __forceinline__ unsigned valid_bits(float v) { return v != v ? 0x7FC00000u : __builtin_bit_cast(unsigned, v); }
@@ -66,97 +72,129 @@ __device__ __forceinline__ void publish(unsigned long long* p, float A, float B)
 __device__ __forceinline__ void publish(unsigned* p, float v) { __hip_atomic_store(p, valid_bits(v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 
 // The value that enters the i-th tile of a chain (i = 0: `first`), for one channel a lane.  slot: the tile's place among the
-// compositions; hop: from one tile of the chain to the next; row: the group's place among the states, row_hop: to the group before.
-__device__ __forceinline__ float look_back(const ScanWs& w, int i, float first, long long slot, long long hop, long long row, long long row_hop) {
+// compositions (of the workgroup: the same for all lanes); hop: from one tile of the chain to the next; row: the group's place among
+// the states, row_hop: to the group before.
+__device__ __forceinline__ float look_back(const ScanWs& w, int i, float first, unsigned lane, long long slot, long long hop, long long row, long long row_hop) {
     if (i == 0) return first;
     const bool head = i % SCAN_GROUP == 0;             // the first tile of a group folds the whole group before it
     const int m = head ? SCAN_GROUP : i % SCAN_GROUP, group = i / SCAN_GROUP - (head ? 1 : 0);
     const unsigned* start = w.state + (head ? row - row_hop : row);
     const unsigned long long* from = w.piece + (slot - hop * m);
-    unsigned long long pc[SCAN_GROUP];
-    unsigned st = 0;
     const unsigned long long t0 = __builtin_amdgcn_s_memrealtime();
+    unsigned st = 0;
+    unsigned long long pc[SCAN_GROUP];
     for (;;) {
-        bool there = true;
-        if (group > 0) { st = __hip_atomic_load(start, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); there = st != ~0u; }
+        // all of it at once, each address a scalar base and the lane
+        if (group > 0) st = __hip_atomic_load(start + lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 #pragma unroll
-        for (int k = 0; k < SCAN_GROUP; ++k) pc[k] = __hip_atomic_load(from + hop * (k < m ? k : m - 1), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        for (int k = 0; k < SCAN_GROUP; ++k) {
+            const unsigned long long* at = from + hop * (k < m ? k : m - 1);
+            asm("" : "+s"(at));
+            pc[k] = __hip_atomic_load(at + lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        bool there = st != ~0u;
 #pragma unroll
         for (int k = 0; k < SCAN_GROUP; ++k) there = there && pc[k] != ~0ull;
-        if (!__any(!there)) break;
-        if (__builtin_amdgcn_s_memrealtime() - t0 > SCAN_WAIT_TICKS) { first = __builtin_nanf(""); st = 0x7FC00000u; break; }
+        if (__all(there)) break;
+        // not yet: wait for the tile before, then for the state, one word a lane at a time (waves that wait would otherwise read as
+        // much as waves that work)
+        const unsigned long long* before = w.piece + (slot - hop);
+        bool wait = true;
+        while (wait) {
+            __builtin_amdgcn_s_sleep(1);
+            const unsigned long long v = __hip_atomic_load(before + lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            wait = !__all(v != ~0ull);
+            if (!wait && group > 0) wait = !__all(__hip_atomic_load(start + lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != ~0u);
+            if (__builtin_amdgcn_s_memrealtime() - t0 > SCAN_WAIT_TICKS) return __builtin_nanf("");
+        }
     }
     float h = group > 0 ? __builtin_bit_cast(float, st) : first;
 #pragma unroll
     for (int k = 0; k < SCAN_GROUP; ++k)
         if (k < m) h = fmaf(__builtin_bit_cast(float, (unsigned)pc[k]), h, __builtin_bit_cast(float, (unsigned)(pc[k] >> 32)));
-    if (head) publish(w.state + row, h);
+    if (head) publish(w.state + row + lane, h);
     return h;
 }
 
-struct TileIds { int tile, b, c0, len; long long chain, chains; };
+struct TileIds { int tile, b, c0, len; unsigned chain, chains; };
 
-template <int C>
+template <int CH>
 __device__ __forceinline__ TileIds tile_ids(const t2_scan_args& a, const ScanWs& w, int ntile, bool from_end) {
-    __shared__ unsigned s_id;
-    unsigned id = blockIdx.x;
-    if (ntile > 1) {
-        if (threadIdx.x == 0) s_id = atomicAdd(w.next, 1u);
-        __syncthreads();
-        id = s_id;
-    }
+    __shared__ unsigned s_tile;
     TileIds t;
-    const int ncb = (a.H + SCAN_CH - 1) / SCAN_CH;
-    t.chains = (long long)a.B * ncb;
-    t.tile = (int)(id / (unsigned)t.chains);
-    t.chain = id - (unsigned)t.tile * (unsigned)t.chains;
-    t.b = (int)(t.chain / ncb);
-    t.c0 = (int)(t.chain - (long long)t.b * ncb) * SCAN_CH;
+    const int ncb = (a.H + CH - 1) / CH;
+    t.chains = (unsigned)a.B * (unsigned)ncb;
+    t.chain = blockIdx.x % t.chains;
+    t.tile = 0;
+    if (ntile > 1) {
+        if (threadIdx.x == 0) s_tile = atomicAdd(w.next + (size_t)t.chain * 16, 1u);
+        __syncthreads();
+        t.tile = __builtin_amdgcn_readfirstlane((int)s_tile);
+    }
+    t.b = (int)(t.chain / (unsigned)ncb);
+    t.c0 = (int)(t.chain - (unsigned)t.b * (unsigned)ncb) * CH;
     if (from_end) t.tile = ntile - 1 - t.tile;
     t.len = row_length(a.lens, t.b, a.T);
     return t;
 }
 
-// L rows of four channels; rows at or behind the row's length repeat its last position (discarded by the caller)
-template <typename E, bool VEC, int L>
-__device__ __forceinline__ void load_rows(typename E::Raw* r, const t2_seq& q, int b, int c, int nc, int s0, int len, bool reverse) {
-    const int last = len > 0 ? len - 1 : 0;
-    const long long base = (long long)b * q.stride_b + c, dt = reverse ? -q.stride_t : q.stride_t;
-    const long long first = base + (long long)(reverse ? last : 0) * q.stride_t;
-    if (s0 + L <= len) {
-        long long at = first + (long long)s0 * dt;
+// zeros at the positions of the tile that lie behind the row's length
+template <typename E, bool BUF, int L>
+__device__ __forceinline__ void zero_rows(const t2_seq& q, int b, int first, int tg, int c, int nc, bool on, int len, int T) {
+    const int rows = T - first;                              // a tile's rows never reach beyond this
+    const SeqRows<E, BUF> r(q, b, first, rows, len, false);
 #pragma unroll
-        for (int l = 0; l < L; ++l, at += dt) r[l] = load4<E, VEC>(q.ptr, at, nc);
-    } else {
-#pragma unroll
-        for (int l = 0; l < L; ++l) r[l] = load4<E, VEC>(q.ptr, first + (long long)(s0 + l < last ? s0 + l : last) * dt, nc);
+    for (int l = 0; l < L; ++l) {
+        const int i = tg * L + l;
+        r.template store<false>(i, c, nc, on && first + i >= len && i < rows, 0.f, 0.f, 0.f, 0.f);
     }
 }
 
-template <typename E, bool VEC, int L>
-__device__ __forceinline__ void zero_rows(const t2_seq& q, int b, int c, int nc, int s0, int from, int T) {
-#pragma unroll
-    for (int l = 0; l < L; ++l)
-        if (s0 + l >= from && s0 + l < T) store4<E, VEC>((void*)q.ptr, (long long)b * q.stride_b + (long long)(s0 + l) * q.stride_t + c, nc, 0.f, 0.f, 0.f, 0.f);
+// The channels of a thread: four from c on.  BUF: the last four of the row for threads beyond its end (they repeat another thread's
+// work; `mine`: whether any of them is this thread's to write).  Otherwise nc of them are there.
+struct Channels { int c, nc; bool mine; };
+template <bool BUF>
+__device__ __forceinline__ Channels channels(int c, int H) {
+    Channels r;
+    r.mine = c < H;
+    r.c = BUF ? (c < H - 4 ? c : H - 4) : c;
+    r.nc = BUF ? 4 : c >= H ? 0 : H - c < 4 ? H - c : 4;
+    return r;
+}
+// the channel behind slot `lane` of the tile's channels, or -1
+template <bool BUF>
+__device__ __forceinline__ int channel_of(int c0, unsigned lane_, int H) {
+    const int lane = (int)lane_;
+    if (BUF) { const int c = c0 + (lane & ~3); return (c < H - 4 ? c : H - 4) + (lane & 3); }
+    return c0 + lane < H ? c0 + lane : -1;
 }
 
-template <typename E, bool GATE, bool VEC, int TG, int L>
-__global__ __launch_bounds__(16 * TG) void scan_tile_kernel(t2_scan_args a, ScanWs w, int ntile) {
-    constexpr int C = TG * L;
-    __shared__ float2 s_piece[TG][SCAN_CH];
-    __shared__ f32v4 s_in[TG][SCAN_CH / 4];
-    const TileIds t = tile_ids<C>(a, w, ntile, false);
-    const int len = t.len, tg = threadIdx.x >> 4, ch = (threadIdx.x & 15) * 4, s0 = t.tile * C + tg * L;
-    // lanes beyond the last channel repeat it and store nothing
-    const int here = a.H - (t.c0 + ch), c = here > 0 ? t.c0 + ch : (VEC ? a.H - 4 : a.H - 1), nc = here > 4 ? 4 : here > 0 ? here : 1;
-    if (t.tile * C >= len && t.tile > 0) {
-        if (here > 0) zero_rows<E, VEC, L>(a.y, t.b, c, nc, s0, len, a.T);
+template <typename E, bool GATE, bool BUF, bool NT, int LANES, int TG, int L, int WAVES>
+__global__ __launch_bounds__(LANES* TG, WAVES) void scan_tile_kernel(t2_scan_args a, ScanWs w, int ntile) {
+    constexpr int C = TG * L, CH = 4 * LANES;
+    __shared__ float2 s_piece[TG][CH];
+    __shared__ f32v4 s_in[TG][LANES];
+    const TileIds t = tile_ids<CH>(a, w, ntile, false);
+    const int len = t.len, tg = threadIdx.x / LANES, first = t.tile * C, i0 = tg * L, s0 = first + i0;
+    const Channels me = channels<BUF>(t.c0 + (threadIdx.x % LANES) * 4, a.H);
+    if (first >= len && t.tile > 0) {
+        zero_rows<E, BUF, L>(a.y, t.b, first, tg, me.c, me.nc, me.mine, len, a.T);
         return;
     }
+    const int rows = len - first < C ? len - first : C;      // steps that are there: rows - 1 is the tile's last (0: an empty row)
     typename E::Raw zr[L], fr[L], orr[L];
-    load_rows<E, VEC, L>(fr, a.f, t.b, c, nc, s0, len, a.reverse);
-    load_rows<E, VEC, L>(zr, a.z, t.b, c, nc, s0, len, a.reverse);
-    if (GATE) load_rows<E, VEC, L>(orr, a.o, t.b, c, nc, s0, len, a.reverse);
+    {
+        const SeqRows<E, BUF> f(a.f, t.b, first, rows, len, a.reverse), z(a.z, t.b, first, rows, len, a.reverse);
+#pragma unroll
+        for (int l = 0; l < L; ++l) fr[l] = f.load(i0 + l, me.c, me.nc, i0 + l < rows);
+#pragma unroll
+        for (int l = 0; l < L; ++l) zr[l] = z.load(i0 + l, me.c, me.nc, i0 + l < rows);
+    }
+    if (GATE) {
+        const SeqRows<E, BUF> o(a.o, t.b, first, rows, len, a.reverse);
+#pragma unroll
+        for (int l = 0; l < L; ++l) orr[l] = o.load(i0 + l, me.c, me.nc, i0 + l < rows);
+    }
     float ga[L][4], x[L][4], A[4] = {1.f, 1.f, 1.f, 1.f}, B[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int l = 0; l < L; ++l)
@@ -166,11 +204,11 @@ __global__ __launch_bounds__(16 * TG) void scan_tile_kernel(t2_scan_args a, Scan
             gate(E::at(fr[l], j), ga[l][j], b);
             x[l][j] = b * E::at(zr[l], j);
         }
-    if (s0 + L > len) {                                      // padding: h stays
+    if (rows < C) {                                          // padding: h stays
 #pragma unroll
         for (int l = 0; l < L; ++l)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) if (s0 + l >= len) { ga[l][j] = 1.f; x[l][j] = 0.f; }
+            for (int j = 0; j < 4; ++j) if (i0 + l >= rows) { ga[l][j] = 1.f; x[l][j] = 0.f; }
     }
 #pragma unroll
     for (int l = 0; l < L; ++l)
@@ -180,78 +218,87 @@ __global__ __launch_bounds__(16 * TG) void scan_tile_kernel(t2_scan_args a, Scan
             A[j] *= ga[l][j];
         }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) s_piece[tg][ch + j] = make_float2(A[j], B[j]);
+    for (int j = 0; j < 4; ++j) s_piece[tg][(threadIdx.x % LANES) * 4 + j] = make_float2(A[j], B[j]);
     __syncthreads();
-    if (threadIdx.x < SCAN_CH) {
-        const int lane = threadIdx.x, cc = t.c0 + lane;
-        float2 p[TG];
+    if (threadIdx.x < CH) {
+        const unsigned lane = threadIdx.x;
+        const int cc = channel_of<BUF>(t.c0, lane, a.H);
         float At = 1.f, Bt = 0.f;
 #pragma unroll
         for (int i = 0; i < TG; ++i) {
-            p[i] = s_piece[i][lane];
-            Bt = fmaf(p[i].x, Bt, p[i].y);
-            At *= p[i].x;
+            const float2 p = s_piece[i][lane];
+            Bt = fmaf(p.x, Bt, p.y);
+            At *= p.x;
         }
-        const long long slot = (t.tile * t.chains + t.chain) * SCAN_CH + lane;
-        const bool more = (t.tile + 1) * C < len;               // a tile behind this one will look back
-        if (more) publish(w.piece + slot, At, Bt);
-        const long long line = t.chains * SCAN_CH, row = (t.tile / SCAN_GROUP) * line + t.chain * SCAN_CH + lane;
-        float h = look_back(w, t.tile, a.state && cc < a.H ? a.state[(long long)t.b * a.H + cc] : 0.f, slot, line, row, line);
-        if (!more && a.final_state && cc < a.H) a.final_state[(long long)t.b * a.H + cc] = fmaf(At, h, Bt);
+        const long long line = (long long)t.chains * CH, place = (long long)t.chain * CH, slot = t.tile * line + place;
+        const bool more = first + C < len;                       // a tile behind this one will look back
+        if (more) publish(w.piece + slot + lane, At, Bt);
+        float h = look_back(w, t.tile, a.state && cc >= 0 ? a.state[(long long)t.b * a.H + cc] : 0.f, lane, slot, line, t.tile / SCAN_GROUP * line + place, line);
+        asm volatile("" ::: "memory");                         // the pieces are read again, not kept in 2 TG registers meanwhile
+        if (!more && a.final_state && cc >= 0) a.final_state[(long long)t.b * a.H + cc] = fmaf(At, h, Bt);
 #pragma unroll
         for (int i = 0; i < TG; ++i) {
+            const float2 p = s_piece[i][lane];
             ((float*)s_in[i])[lane] = h;
-            h = fmaf(p[i].x, h, p[i].y);
+            h = fmaf(p.x, h, p.y);
         }
     }
     __syncthreads();
-    if (here <= 0) return;
-    const f32v4 hin = s_in[tg][threadIdx.x & 15];
+    const f32v4 hin = s_in[tg][threadIdx.x % LANES];
     float h[4] = {hin[0], hin[1], hin[2], hin[3]};
-    if (a.tape && s0 < len && s0 % T2_SCAN_SPAN == 0) {
-        float* q = a.tape + ((long long)t.b * ((a.T + T2_SCAN_SPAN - 1) / T2_SCAN_SPAN) + s0 / T2_SCAN_SPAN) * a.H + c;
-        for (int j = 0; j < nc; ++j) q[j] = h[j];
-    }
-    const long long dt = a.reverse ? -a.y.stride_t : a.y.stride_t;
-    long long at = (long long)t.b * a.y.stride_b + c + (long long)(a.reverse ? len - 1 - s0 : s0) * a.y.stride_t;
+    if (a.tape && i0 < rows && s0 % T2_SCAN_SPAN == 0 && me.mine) {
+        float* q = a.tape + ((long long)t.b * ((a.T + T2_SCAN_SPAN - 1) / T2_SCAN_SPAN) + s0 / T2_SCAN_SPAN) * a.H + me.c;
 #pragma unroll
-    for (int l = 0; l < L; ++l, at += dt) {
+        for (int j = 0; j < 4; ++j) if (j < me.nc) q[j] = h[j];
+    }
+    const SeqRows<E, BUF> out(a.y, t.b, first, rows, len, a.reverse);
+#pragma unroll
+    for (int l = 0; l < L; ++l) {
         float y[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             h[j] = fmaf(ga[l][j], h[j], x[l][j]);
             y[j] = GATE ? h[j] * sigmoid1(E::at(orr[l], j)) : h[j];
         }
-        if (s0 + l < len) store4<E, VEC>((void*)a.y.ptr, at, nc, y[0], y[1], y[2], y[3]);
+        out.template store<NT>(i0 + l, me.c, me.nc, i0 + l < rows && me.mine, y[0], y[1], y[2], y[3]);
     }
-    if (s0 + L > len) zero_rows<E, VEC, L>(a.y, t.b, c, nc, s0, len, a.T);
+    if (rows < C) zero_rows<E, BUF, L>(a.y, t.b, first, tg, me.c, me.nc, me.mine, len, a.T);
 }
 
 // Backward: l_t = the gradient that leaves step t for the state in front of it obeys l_t = a_t (l_{t+1} + g_t), g = dy sigmoid(o), the same
 // recurrence from the other end; tiles are drawn from the last to the first and look back at the tiles behind them.  The states inside
 // the tile come from the tape's, which needs no other tile.
-template <typename E, bool GATE, bool VEC, int TG, int L>
-__global__ __launch_bounds__(16 * TG) void scan_tile_backward_kernel(t2_scan_args a, ScanWs w, int ntile) {
-    constexpr int C = TG * L;
+template <typename E, bool GATE, bool BUF, bool NT, int LANES, int TG, int L, int WAVES>
+__global__ __launch_bounds__(LANES* TG, WAVES) void scan_tile_backward_kernel(t2_scan_args a, ScanWs w, int ntile) {
+    constexpr int C = TG * L, CH = 4 * LANES;
     static_assert(C % T2_SCAN_SPAN == 0 && T2_SCAN_SPAN % L == 0, "tiles start where the tape has a state");
-    __shared__ float2 s_fwd[TG][SCAN_CH], s_bwd[TG][SCAN_CH];
-    __shared__ f32v4 s_h[TG][SCAN_CH / 4], s_l[TG][SCAN_CH / 4];
-    const TileIds t = tile_ids<C>(a, w, ntile, true);
-    const int len = t.len, tg = threadIdx.x >> 4, ch = (threadIdx.x & 15) * 4, s0 = t.tile * C + tg * L;
-    const int here = a.H - (t.c0 + ch), c = here > 0 ? t.c0 + ch : (VEC ? a.H - 4 : a.H - 1), nc = here > 4 ? 4 : here > 0 ? here : 1;
-    if (t.tile * C >= len && t.tile > 0) {
-        if (here > 0) {
-            zero_rows<E, VEC, L>(a.dz, t.b, c, nc, s0, len, a.T);
-            zero_rows<E, VEC, L>(a.df, t.b, c, nc, s0, len, a.T);
-            if (GATE) zero_rows<E, VEC, L>(a.do_, t.b, c, nc, s0, len, a.T);
-        }
-        return;
-    }
+    __shared__ float2 s_fwd[TG][CH], s_bwd[TG][CH];
+    __shared__ f32v4 s_h[TG][LANES], s_l[TG][LANES];
+    const TileIds t = tile_ids<CH>(a, w, ntile, true);
+    const int len = t.len, tg = threadIdx.x / LANES, first = t.tile * C, i0 = tg * L;
+    const Channels me = channels<BUF>(t.c0 + (threadIdx.x % LANES) * 4, a.H);
+    auto zeros = [&] {
+        zero_rows<E, BUF, L>(a.dz, t.b, first, tg, me.c, me.nc, me.mine, len, a.T);
+        zero_rows<E, BUF, L>(a.df, t.b, first, tg, me.c, me.nc, me.mine, len, a.T);
+        if (GATE) zero_rows<E, BUF, L>(a.do_, t.b, first, tg, me.c, me.nc, me.mine, len, a.T);
+    };
+    if (first >= len && t.tile > 0) { zeros(); return; }
+    const int rows = len - first < C ? len - first : C;
     typename E::Raw zr[L], fr[L], orr[L], dr[L];
-    load_rows<E, VEC, L>(fr, a.f, t.b, c, nc, s0, len, a.reverse);
-    load_rows<E, VEC, L>(zr, a.z, t.b, c, nc, s0, len, a.reverse);
-    load_rows<E, VEC, L>(dr, a.dy, t.b, c, nc, s0, len, a.reverse);
-    if (GATE) load_rows<E, VEC, L>(orr, a.o, t.b, c, nc, s0, len, a.reverse);
+    {
+        const SeqRows<E, BUF> f(a.f, t.b, first, rows, len, a.reverse), z(a.z, t.b, first, rows, len, a.reverse), d(a.dy, t.b, first, rows, len, a.reverse);
+#pragma unroll
+        for (int l = 0; l < L; ++l) fr[l] = f.load(i0 + l, me.c, me.nc, i0 + l < rows);
+        if (GATE) {
+            const SeqRows<E, BUF> o(a.o, t.b, first, rows, len, a.reverse);
+#pragma unroll
+            for (int l = 0; l < L; ++l) orr[l] = o.load(i0 + l, me.c, me.nc, i0 + l < rows);
+        }
+#pragma unroll
+        for (int l = 0; l < L; ++l) dr[l] = d.load(i0 + l, me.c, me.nc, i0 + l < rows);
+#pragma unroll
+        for (int l = 0; l < L; ++l) zr[l] = z.load(i0 + l, me.c, me.nc, i0 + l < rows);
+    }
     float ga[L][4], gb[L][4], g[L][4], gn[GATE ? L : 1][4];        // gn: g (1 - sigmoid(o)), do but for h
     float A[4] = {1.f, 1.f, 1.f, 1.f}, B[4] = {0.f, 0.f, 0.f, 0.f}, Q[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -259,16 +306,25 @@ __global__ __launch_bounds__(16 * TG) void scan_tile_backward_kernel(t2_scan_arg
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             gate(E::at(fr[l], j), ga[l][j], gb[l][j]);
-            g[l][j] = E::at(dr[l], j);
-            float z = E::at(zr[l], j);
+            g[l][j] = E::at(dr[l], j);                             // rows that are not there were read as zeros
             if (GATE) {
                 float so, sn;
                 gate(E::at(orr[l], j), so, sn);
                 g[l][j] *= so;
                 gn[l][j] = g[l][j] * sn;
             }
-            if (s0 + l >= len) { ga[l][j] = 1.f; gb[l][j] = 0.f; g[l][j] = 0.f; z = 0.f; }
-            B[j] = fmaf(ga[l][j], B[j], gb[l][j] * z);
+        }
+    if (rows < C) {
+#pragma unroll
+        for (int l = 0; l < L; ++l)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) if (i0 + l >= rows) { ga[l][j] = 1.f; gb[l][j] = 0.f; }
+    }
+#pragma unroll
+    for (int l = 0; l < L; ++l)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            B[j] = fmaf(ga[l][j], B[j], gb[l][j] * E::at(zr[l], j));
             A[j] *= ga[l][j];
         }
 #pragma unroll
@@ -277,49 +333,55 @@ __global__ __launch_bounds__(16 * TG) void scan_tile_backward_kernel(t2_scan_arg
         for (int j = 0; j < 4; ++j) Q[j] = ga[l][j] * (Q[j] + g[l][j]);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        s_fwd[tg][ch + j] = make_float2(A[j], B[j]);
-        s_bwd[tg][ch + j] = make_float2(A[j], Q[j]);
+        const int k = (threadIdx.x % LANES) * 4 + j;
+        s_fwd[tg][k] = make_float2(A[j], B[j]);
+        s_bwd[tg][k] = make_float2(A[j], Q[j]);
     }
     __syncthreads();
-    if (threadIdx.x < SCAN_CH) {                                   // one wave: the states, from the tape's
-        const int lane = threadIdx.x, cc = t.c0 + lane, ntape = (a.T + T2_SCAN_SPAN - 1) / T2_SCAN_SPAN;
+    if (threadIdx.x < CH) {                                        // the states, from the tape's
+        const unsigned lane = threadIdx.x;
+        const int cc = channel_of<BUF>(t.c0, lane, a.H), ntape = (a.T + T2_SCAN_SPAN - 1) / T2_SCAN_SPAN;
         const float* tape = a.tape + ((long long)t.b * ntape + t.tile * (C / T2_SCAN_SPAN)) * a.H + cc;
         float h = 0.f;
 #pragma unroll
         for (int i = 0; i < TG; ++i) {
             const int j = i * L / T2_SCAN_SPAN;
-            if (i * L % T2_SCAN_SPAN == 0) h = cc < a.H && t.tile * C + j * T2_SCAN_SPAN < len ? tape[(long long)j * a.H] : 0.f;
+            if (i * L % T2_SCAN_SPAN == 0) h = cc >= 0 && j * T2_SCAN_SPAN < rows ? tape[(long long)j * a.H] : 0.f;
+            const float2 p = s_fwd[i][lane];
             ((float*)s_h[i])[lane] = h;
-            h = fmaf(s_fwd[i][lane].x, h, s_fwd[i][lane].y);
+            h = fmaf(p.x, h, p.y);
         }
-    } else if (threadIdx.x < 2 * SCAN_CH) {                        // another: the gradients that enter
-        const int lane = threadIdx.x - SCAN_CH, cc = t.c0 + lane;
-        float2 p[TG];
+    }
+    constexpr int SIDE = TG >= 8 ? CH : 0;                         // other waves where there are some: the gradients that enter
+    if (threadIdx.x >= SIDE && threadIdx.x < SIDE + CH) {
+        const unsigned lane = threadIdx.x - SIDE;
+        const int cc = channel_of<BUF>(t.c0, lane, a.H);
         float At = 1.f, Qt = 0.f;
 #pragma unroll
         for (int i = TG - 1; i >= 0; --i) {
-            p[i] = s_bwd[i][lane];
-            Qt = fmaf(p[i].x, Qt, p[i].y);
-            At *= p[i].x;
+            const float2 p = s_bwd[i][lane];
+            Qt = fmaf(p.x, Qt, p.y);
+            At *= p.x;
         }
-        const long long slot = (t.tile * t.chains + t.chain) * SCAN_CH + lane;
-        const int last = len > 0 ? (len - 1) / C : 0;              // the last tile that is not all padding
-        if (t.tile > 0) publish(w.piece + slot, At, Qt);
-        const long long line = t.chains * SCAN_CH, row = ((last - t.tile) / SCAN_GROUP) * line + t.chain * SCAN_CH + lane;
-        float l = look_back(w, last - t.tile, a.dfinal && cc < a.H ? a.dfinal[(long long)t.b * a.H + cc] : 0.f, slot, -line, row, line);
-        if (t.tile == 0 && a.dstate && cc < a.H) a.dstate[(long long)t.b * a.H + cc] = fmaf(At, l, Qt);
+        const int last = len > 0 ? (len - 1) / C : 0, at = last - t.tile;       // the last tile that is not all padding comes first
+        const long long line = (long long)t.chains * CH, place = (long long)t.chain * CH, slot = t.tile * line + place;
+        if (t.tile > 0) publish(w.piece + slot + lane, At, Qt);
+        float l = look_back(w, at, a.dfinal && cc >= 0 ? a.dfinal[(long long)t.b * a.H + cc] : 0.f, lane, slot, -line, at / SCAN_GROUP * line + place, line);
+        asm volatile("" ::: "memory");
+        if (t.tile == 0 && a.dstate && cc >= 0) a.dstate[(long long)t.b * a.H + cc] = fmaf(At, l, Qt);
 #pragma unroll
         for (int i = TG - 1; i >= 0; --i) {
+            const float2 p = s_bwd[i][lane];
             ((float*)s_l[i])[lane] = l;
-            l = fmaf(p[i].x, l, p[i].y);
+            l = fmaf(p.x, l, p.y);
         }
     }
     __syncthreads();
-    if (here <= 0) return;
-    const f32v4 hin = s_h[tg][threadIdx.x & 15], lin = s_l[tg][threadIdx.x & 15];
+    const f32v4 hin = s_h[tg][threadIdx.x % LANES], lin = s_l[tg][threadIdx.x % LANES];
     float h[4] = {hin[0], hin[1], hin[2], hin[3]}, d[4] = {lin[0], lin[1], lin[2], lin[3]};
-    const long long t0 = a.reverse ? len - 1 - s0 : s0, sign = a.reverse ? -1 : 1;
     float wf[L][4];                                                // df but for the gradient of h
+    const SeqRows<E, BUF> dz(a.dz, t.b, first, rows, len, a.reverse), df(a.df, t.b, first, rows, len, a.reverse);
+    const SeqRows<E, BUF> dout(GATE ? a.do_ : a.dz, t.b, first, rows, len, a.reverse);
 #pragma unroll
     for (int l = 0; l < L; ++l) {
         float o4[4];
@@ -330,8 +392,7 @@ __global__ __launch_bounds__(16 * TG) void scan_tile_backward_kernel(t2_scan_arg
             h[j] = fmaf(ga[l][j], h[j], gb[l][j] * z);
             if (GATE) o4[j] = gn[l][j] * h[j];
         }
-        if (GATE && s0 + l < len)
-            store4<E, VEC>((void*)a.do_.ptr, (long long)t.b * a.do_.stride_b + c + (t0 + sign * l) * a.do_.stride_t, nc, o4[0], o4[1], o4[2], o4[3]);
+        if (GATE) dout.template store<NT>(i0 + l, me.c, me.nc, i0 + l < rows && me.mine, o4[0], o4[1], o4[2], o4[3]);
     }
 #pragma unroll
     for (int l = L - 1; l >= 0; --l) {
@@ -343,16 +404,10 @@ __global__ __launch_bounds__(16 * TG) void scan_tile_backward_kernel(t2_scan_arg
             f4[j] = wf[l][j] * d[j];
             d[j] *= ga[l][j];
         }
-        if (s0 + l < len) {
-            store4<E, VEC>((void*)a.dz.ptr, (long long)t.b * a.dz.stride_b + c + (t0 + sign * l) * a.dz.stride_t, nc, z4[0], z4[1], z4[2], z4[3]);
-            store4<E, VEC>((void*)a.df.ptr, (long long)t.b * a.df.stride_b + c + (t0 + sign * l) * a.df.stride_t, nc, f4[0], f4[1], f4[2], f4[3]);
-        }
+        dz.template store<NT>(i0 + l, me.c, me.nc, i0 + l < rows && me.mine, z4[0], z4[1], z4[2], z4[3]);
+        df.template store<NT>(i0 + l, me.c, me.nc, i0 + l < rows && me.mine, f4[0], f4[1], f4[2], f4[3]);
     }
-    if (s0 + L > len) {
-        zero_rows<E, VEC, L>(a.dz, t.b, c, nc, s0, len, a.T);
-        zero_rows<E, VEC, L>(a.df, t.b, c, nc, s0, len, a.T);
-        if (GATE) zero_rows<E, VEC, L>(a.do_, t.b, c, nc, s0, len, a.T);
-    }
+    if (rows < C) zeros();
 }
 
 struct StepArgs {
@@ -386,19 +441,47 @@ extern "C" int64_t t2_gated_scan_tape(int B, int T, int H) {
     return (int64_t)B * ((T + T2_SCAN_SPAN - 1) / T2_SCAN_SPAN) * H;
 }
 
-// Steps of a tile (16 lanes x TG threads of L steps)
-template <bool BACKWARD> static int tile_steps(int T) { return BACKWARD ? (T <= 64 ? 64 : T <= 256 ? 256 : 64) : (T <= 64 ? 64 : 256); }
+// The tile of a call, by its sizes (kernel times in us; frames: B=32, T=800, H=512 bf16; long: B=2, T=65536, H=1024 bf16; odd: B=2,
+// T=32769, H=1001 fp16).  A sequence that one tile covers needs no workspace, no look back and one launch: tiles of 64 and of 256
+// steps (B=32, T=140, H=256 fp32: a call of 14 us, 18.6 with two tiles).  Otherwise 64 channels a tile, which gives more and
+// smaller workgroups, and 128 (256 bytes of a 16-bit row) where there are enough of those for 12 and more on every compute unit:
+// forward 20.4 narrow / 24.0 wide at frames, 251 / 237 at long, 165 / 151 at odd; backward 38.6 / 41.2 at frames, 294 / 277 at odd.
+struct Tile {
+    int lanes, tg, l;
+    constexpr int steps() const { return tg * l; }
+    constexpr int channels() const { return 4 * lanes; }
+};
+enum Shape { SHORT, MEDIUM, NARROW, WIDE };
+static constexpr Tile forward_tile[] = {{16, 8, 8}, {16, 32, 8}, {16, 16, 8}, {32, 8, 16}};
+static constexpr Tile backward_tile[] = {{16, 16, 4}, {16, 32, 8}, {16, 16, 4}, {32, 8, 8}};
+static constexpr int forward_waves[] = {4, 4, 4, 2}, backward_waves[] = {3, 2, 3, 2};     // a SIMD: registers for the tile without spills
 
-static int64_t ws_bytes(int B, int T, int H, int steps) {
-    const int64_t ntile = (T + steps - 1) / steps, chains = (int64_t)B * ((H + SCAN_CH - 1) / SCAN_CH);
+static Shape shape_of(bool backward, int B, int T, int H, bool buf) {
+    if (!buf) return NARROW;
+    const Tile* tiles = backward ? backward_tile : forward_tile;
+    if (T <= tiles[SHORT].steps()) return SHORT;
+    if (T <= tiles[MEDIUM].steps()) return MEDIUM;
+    const Tile& w = tiles[WIDE];
+    const int64_t blocks = (int64_t)B * ((H + w.channels() - 1) / w.channels()) * ((T + w.steps() - 1) / w.steps());
+    return blocks >= 12 * 256 ? WIDE : NARROW;
+}
+
+static int64_t ws_bytes(int B, int T, int H, Tile t) {
+    const int64_t ntile = (T + t.steps() - 1) / t.steps(), chains = (int64_t)B * ((H + t.channels() - 1) / t.channels());
     if (ntile * chains > 0x7FFFFFFF) return fail(T2_EINVAL, "[%d,%d,%d] is too large for one call", B, T, H);
-    return ntile < 2 ? 0 : 16 + (ntile * 8 + (ntile + SCAN_GROUP - 1) / SCAN_GROUP * 4) * chains * SCAN_CH;
+    return ntile < 2 ? 0 : chains * 64 + (ntile * 8 + (ntile + SCAN_GROUP - 1) / SCAN_GROUP * 4) * chains * t.channels();
 }
 
 extern "C" int64_t t2_gated_scan_ws(int B, int T, int H) {
     if (!sizes_ok(B, T, H)) return fail(T2_EINVAL, "bad shape [%d,%d,%d]", B, T, H);
-    const int64_t f = ws_bytes(B, T, H, tile_steps<false>(T)), g = ws_bytes(B, T, H, tile_steps<true>(T));
-    return f < 0 || g < 0 ? T2_EINVAL : f > g ? f : g;
+    int64_t most = 0;
+    for (int backward = 0; backward < 2; ++backward)
+        for (int buf = 0; buf < 2; ++buf) {
+            const int64_t n = ws_bytes(B, T, H, (backward ? backward_tile : forward_tile)[shape_of(backward, B, T, H, buf)]);
+            if (n < 0) return n;
+            most = n > most ? n : most;
+        }
+    return most;
 }
 
 static int check_args(const t2_ctx* ctx, const t2_scan_args* a, bool backward) {
@@ -415,59 +498,73 @@ static int check_args(const t2_ctx* ctx, const t2_scan_args* a, bool backward) {
     return T2_OK;
 }
 
-// Vector accesses need whole groups of four channels and rows that start at a multiple of four elements' size.
-static bool vectors(const t2_scan_args* a, const t2_seq* const* q, int n) {
-    const int size = a->dtype == T2_F32 ? 4 : 2;
-    if (a->H % 4 != 0) return false;
+// Buffer descriptors and four channels at a time, but for rows of fewer channels and for strides whose tile leaves the range of an offset.
+static bool buffers(const t2_scan_args* a, int steps, const t2_seq* const* q, int n) {
+    const int64_t size = a->dtype == T2_F32 ? 4 : 2, most = SEQ_RANGE / size / (steps + 1);
+    if (a->H < 4 || a->H > most) return false;
     for (int i = 0; i < n; ++i)
-        if (q[i]->ptr && ((uintptr_t)q[i]->ptr % (4 * size) != 0 || q[i]->stride_b % 4 != 0 || q[i]->stride_t % 4 != 0)) return false;
+        if (q[i]->ptr && (q[i]->stride_t > most || q[i]->stride_t < -most)) return false;
     return true;
 }
 
-template <typename E, bool GATE, bool VEC, bool BACKWARD, int TG, int L>
-static int launch_tiles(t2_ctx* ctx, const t2_scan_args* a) {
-    const int ntile = (a->T + TG * L - 1) / (TG * L);
-    const int64_t blocks = (int64_t)ntile * a->B * ((a->H + SCAN_CH - 1) / SCAN_CH);
+template <typename E, bool GATE, bool BUF, bool NT, bool BACKWARD, Shape S>
+static int launch(t2_ctx* ctx, const t2_scan_args* a) {
+    constexpr Tile tile = BACKWARD ? backward_tile[S] : forward_tile[S];
+    constexpr int CH = tile.channels(), WAVES = BACKWARD ? backward_waves[S] : forward_waves[S];
+    const int ntile = (a->T + tile.steps() - 1) / tile.steps();
+    const int64_t blocks = (int64_t)ntile * a->B * ((a->H + CH - 1) / CH);
     ScanWs w = {};
     if (ntile > 1) {
-        w = scan_ws(a->ws, blocks * SCAN_CH);
-        const long long n16 = ws_bytes(a->B, a->T, a->H, TG * L) / 16, nb = (n16 + 1023) / 1024;
-        hipLaunchKernelGGL(scan_ws_kernel, dim3((unsigned)(nb < 2048 ? nb : 2048)), dim3(256), 0, ctx->stream, (uint4*)a->ws, n16);
+        w = scan_ws(a->ws, blocks / ntile, blocks * CH);
+        const long long n16 = ws_bytes(a->B, a->T, a->H, tile) / 16, nb = (n16 + 1023) / 1024;
+        hipLaunchKernelGGL(scan_ws_kernel, dim3((unsigned)(nb < 2048 ? nb : 2048)), dim3(256), 0, ctx->stream, (uint4*)a->ws, blocks / ntile * 4, n16);
     }
-    if constexpr (BACKWARD) hipLaunchKernelGGL((scan_tile_backward_kernel<E, GATE, VEC, TG, L>), dim3((unsigned)blocks), dim3(16 * TG), 0, ctx->stream, *a, w, ntile);
-    else hipLaunchKernelGGL((scan_tile_kernel<E, GATE, VEC, TG, L>), dim3((unsigned)blocks), dim3(16 * TG), 0, ctx->stream, *a, w, ntile);
+    const dim3 grid((unsigned)blocks), threads(tile.lanes * tile.tg);
+    if constexpr (BACKWARD) hipLaunchKernelGGL((scan_tile_backward_kernel<E, GATE, BUF, NT, tile.lanes, tile.tg, tile.l, WAVES>), grid, threads, 0, ctx->stream, *a, w, ntile);
+    else hipLaunchKernelGGL((scan_tile_kernel<E, GATE, BUF, NT, tile.lanes, tile.tg, tile.l, WAVES>), grid, threads, 0, ctx->stream, *a, w, ntile);
     HIP_TRY(hipGetLastError());
     return T2_OK;
 }
 
-template <typename E, bool GATE, bool VEC, bool BACKWARD>
-static int launch(t2_ctx* ctx, const t2_scan_args* a) {
-    const int steps = tile_steps<BACKWARD>(a->T);
-    if constexpr (BACKWARD) return steps == 64 ? launch_tiles<E, GATE, VEC, true, 16, 4>(ctx, a) : launch_tiles<E, GATE, VEC, true, 64, 4>(ctx, a);
-    else return steps == 64 ? launch_tiles<E, GATE, VEC, false, 8, 8>(ctx, a) : launch_tiles<E, GATE, VEC, false, 32, 8>(ctx, a);
+template <typename E, bool GATE, bool BACKWARD>
+static int launch_shape(t2_ctx* ctx, const t2_scan_args* a, Shape s, bool buf, bool nt) {
+    if (!buf) return launch<E, GATE, false, false, BACKWARD, NARROW>(ctx, a);
+    if (s == SHORT) return launch<E, GATE, true, false, BACKWARD, SHORT>(ctx, a);
+    if (s == MEDIUM) return launch<E, GATE, true, false, BACKWARD, MEDIUM>(ctx, a);
+    if (s == NARROW) return nt ? launch<E, GATE, true, true, BACKWARD, NARROW>(ctx, a) : launch<E, GATE, true, false, BACKWARD, NARROW>(ctx, a);
+    return nt ? launch<E, GATE, true, true, BACKWARD, WIDE>(ctx, a) : launch<E, GATE, true, false, BACKWARD, WIDE>(ctx, a);
 }
 
 template <bool BACKWARD>
-static int launch_any(t2_ctx* ctx, const t2_scan_args* a, bool vec) {
+static int launch_any(t2_ctx* ctx, const t2_scan_args* a, const t2_seq* const* in, int n_in, const t2_seq* const* out, int n_out) {
     DeviceScope dev(ctx->device);
     HIP_TRY(dev.err);
+    // a tile of every shape fits the range of its offsets, or none of this call uses them
+    const Tile& most = (BACKWARD ? backward_tile : forward_tile)[MEDIUM];
+    const bool buf = buffers(a, most.steps(), in, n_in) && buffers(a, most.steps(), out, n_out);
+    const Shape s = shape_of(BACKWARD, a->B, a->T, a->H, buf);
+    // Stores past L2 where they fill whole 128-byte lines (frames: forward 20.9 -> 19.7 us, backward 36.7 -> 32.8); rows that start
+    // inside a line lose by it (odd: backward 290 -> 324).
+    bool nt = true;
+    const int64_t size = a->dtype == T2_F32 ? 4 : 2;
+    for (int i = 0; i < n_out; ++i)
+        if (out[i]->ptr && ((((uintptr_t)out[i]->ptr) | (uintptr_t)(out[i]->stride_b * size) | (uintptr_t)(out[i]->stride_t * size)) & 127)) nt = false;
     const bool gated = a->o.ptr != nullptr;
-#define SCAN_CASE(E) (gated ? vec ? launch<E, true, true, BACKWARD>(ctx, a) : launch<E, true, false, BACKWARD>(ctx, a)                     \
-                            : vec ? launch<E, false, true, BACKWARD>(ctx, a) : launch<E, false, false, BACKWARD>(ctx, a))
+#define SCAN_CASE(E) (gated ? launch_shape<E, true, BACKWARD>(ctx, a, s, buf, nt) : launch_shape<E, false, BACKWARD>(ctx, a, s, buf, nt))
     return a->dtype == T2_F32 ? SCAN_CASE(ElemF32) : a->dtype == T2_BF16 ? SCAN_CASE(ElemBF16) : SCAN_CASE(ElemF16);
 #undef SCAN_CASE
 }
 
 extern "C" int t2_gated_scan(t2_ctx* ctx, const t2_scan_args* a) {
     T2_TRY(check_args(ctx, a, false));
-    const t2_seq* q[] = {&a->z, &a->f, &a->o, &a->y};
-    return launch_any<false>(ctx, a, vectors(a, q, 4));
+    const t2_seq *in[] = {&a->z, &a->f, &a->o}, *out[] = {&a->y};
+    return launch_any<false>(ctx, a, in, 3, out, 1);
 }
 
 extern "C" int t2_gated_scan_backward(t2_ctx* ctx, const t2_scan_args* a) {
     T2_TRY(check_args(ctx, a, true));
-    const t2_seq* q[] = {&a->z, &a->f, &a->o, &a->dy, &a->dz, &a->df, &a->do_};
-    return launch_any<true>(ctx, a, vectors(a, q, 7));
+    const t2_seq *in[] = {&a->z, &a->f, &a->o, &a->dy}, *out[] = {&a->dz, &a->df, &a->do_};
+    return launch_any<true>(ctx, a, in, 4, out, a->o.ptr ? 3 : 2);
 }
 
 extern "C" int t2_gated_scan_step(t2_ctx* ctx, int dtype, int B, int H, const void* z, int64_t z_stride, const void* f, int64_t f_stride, const void* o,
