@@ -15,17 +15,22 @@
 #define AW_THREADS 256
 #define AW_BLOCK 128                 /* elements that share a scale; every tensor's states start at a multiple of it */
 #define AW_VEC 8                     /* elements of a thread: 16 lanes (one DPP row) hold one block */
-#define AW_CHUNK 8192                /* elements of a workgroup */
+#define AW_CHUNK 8192                /* elements of a workgroup (2048: 1.8 M parameters 18.6 us, 17.4 so) */
+// From here on the norm reads gradients past the last-level cache: what it leaves there is gone before the step comes to it, and
+// what it would push out are the step before's results (272 M bf16 gradients: 968 us in all, 948 so; 27 M fp32: 177, 180 so).
+#define AW_STREAM_FROM (128LL << 20)
 #define AW_NORM_BLOCKS 2048
+#define AW_GROUPS 32                 /* of the workgroups of the norm, each with a counter on a line of its own */
 #define AW_STREAM 20                 /* of the counter-based generator */
 #define AW_BIND 96                   /* tensors a binding launch takes by value */
 
 struct AwTensor { long long n, off; float decay; int chunk0; };
 struct AwBound { const void* g; void* p; void* c; uint32_t g_type, p_type, c_type, aligned; };
-struct AwCtl { float gs, lr, lr_t, ic2; uint32_t t; int skip; uint32_t ticket; };
+struct AwCtl { float gs, lr, lr_t, ic2; uint32_t t; int skip; uint32_t pad[10]; uint32_t ticket[(AW_GROUPS + 1) * 16]; };
 
 struct t2_adamw {
     int device = 0, n_tensors = 0, n_chunks = 0, bits = 32;
+    bool stream = false;
     double b1 = 0, b2 = 0, eps = 0;
     uint32_t seed = 0;
     void *m = nullptr, *v = nullptr;
@@ -40,25 +45,34 @@ struct t2_adamw {
 // ------------------------------------------------------------------------------------------------
 // eight neighbouring elements of a tensor of any of the three types (type and alignment are the same for a whole workgroup)
 // ------------------------------------------------------------------------------------------------
+#define AW_GLOBAL __attribute__((address_space(1)))     // addresses out of a table are global memory: the compiler cannot know
+template <typename E, bool STREAM = false>
+__device__ __forceinline__ typename E::Raw load4(const void* p, long long i) {
+    const AW_GLOBAL typename E::Raw* q = (const AW_GLOBAL typename E::Raw*)((const AW_GLOBAL typename E::T*)(uintptr_t)p + i);
+    if constexpr (STREAM) return __builtin_nontemporal_load(q);
+    else return *q;
+}
 template <typename E>
 __device__ __forceinline__ void load8(const void* p, long long i, int n, bool aligned, float* x) {
     if (aligned && n >= AW_VEC) {
-        const typename E::Raw lo = *(const typename E::Raw*)((const typename E::T*)p + i), hi = *(const typename E::Raw*)((const typename E::T*)p + i + 4);
+        const typename E::Raw lo = load4<E>(p, i), hi = load4<E>(p, i + 4);
 #pragma unroll
         for (int j = 0; j < 4; ++j) { x[j] = E::at(lo, j); x[j + 4] = E::at(hi, j); }
     } else {
+        const AW_GLOBAL typename E::T* q = (const AW_GLOBAL typename E::T*)(uintptr_t)p + i;
 #pragma unroll
-        for (int j = 0; j < AW_VEC; ++j) x[j] = j < n ? E::get(p, i + j) : 0.f;
+        for (int j = 0; j < AW_VEC; ++j) x[j] = j < n ? (float)q[j] : 0.f;
     }
 }
 template <typename E>
 __device__ __forceinline__ void store8(void* p, long long i, int n, bool aligned, const float* x) {
+    AW_GLOBAL typename E::T* q = (AW_GLOBAL typename E::T*)(uintptr_t)p + i;
     if (aligned && n >= AW_VEC) {
-        *(typename E::Raw*)((typename E::T*)p + i) = E::pack(x[0], x[1], x[2], x[3]);
-        *(typename E::Raw*)((typename E::T*)p + i + 4) = E::pack(x[4], x[5], x[6], x[7]);
+        *(AW_GLOBAL typename E::Raw*)q = E::pack(x[0], x[1], x[2], x[3]);
+        *(AW_GLOBAL typename E::Raw*)(q + 4) = E::pack(x[4], x[5], x[6], x[7]);
     } else {
 #pragma unroll
-        for (int j = 0; j < AW_VEC; ++j) if (j < n) E::put(p, i + j, x[j]);
+        for (int j = 0; j < AW_VEC; ++j) if (j < n) q[j] = (typename E::T)x[j];
     }
 }
 __device__ __forceinline__ void load8(const void* p, uint32_t type, long long i, int n, bool aligned, float* x) {
@@ -108,23 +122,40 @@ __device__ void begin_step(const AwNormArgs& a, double norm) {
 // Sums of squares in double, so that the clipping factor does not depend on how the work is split; the last workgroup to
 // arrive adds the partial sums in a fixed order.  The sums go through agent-scope accesses that are waited for, not through a
 // fence: a release at agent scope writes back a whole L2 for every workgroup (27 M gradients: 153 us with it).
+template <typename E, bool STREAM>
+__device__ __forceinline__ double chunk_squares(const void* p, long long base, long long n, bool aligned) {
+    constexpr int R = AW_CHUNK / (AW_THREADS * 4);
+    double s = 0.0;
+    if (aligned && base + AW_CHUNK <= n) {                    // all loads of the chunk in flight
+        typename E::Raw r[R];
+#pragma unroll
+        for (int k = 0; k < R; ++k) r[k] = load4<E, STREAM>(p, base + (k * AW_THREADS + (int)threadIdx.x) * 4);
+#pragma unroll
+        for (int k = 0; k < R; ++k)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) { const double x = (double)E::at(r[k], j); s = fma(x, x, s); }
+    } else {
+        const AW_GLOBAL typename E::T* q = (const AW_GLOBAL typename E::T*)(uintptr_t)p;
+        const long long end = base + AW_CHUNK < n ? base + AW_CHUNK : n;
+        for (long long i = base + threadIdx.x; i < end; i += AW_THREADS) { const double x = (double)(float)q[i]; s = fma(x, x, s); }
+    }
+    return s;
+}
+
+template <bool STREAM>
 __global__ __launch_bounds__(AW_THREADS) void adamw_norm_kernel(AwNormArgs a) {
     __shared__ double sh[AW_THREADS / 64];
     __shared__ bool last;
     double s = 0.0;
+    int next = a.chunk_tensor[blockIdx.x];
     for (int chunk = blockIdx.x; chunk < a.n_chunks; chunk += gridDim.x) {
-        const int k = a.chunk_tensor[chunk];
+        const int k = next;
         const AwTensor t = a.tensors[k];
         const AwBound b = a.bound[k];
+        if (chunk + (int)gridDim.x < a.n_chunks) next = a.chunk_tensor[chunk + gridDim.x];
         const long long base = (long long)(chunk - t.chunk0) * AW_CHUNK;
-        for (int it = 0; it < AW_CHUNK / (AW_THREADS * AW_VEC); ++it) {
-            const long long i = base + (it * AW_THREADS + threadIdx.x) * AW_VEC;
-            if (i >= t.n) break;
-            float x[AW_VEC];
-            load8(b.g, b.g_type, i, (int)(t.n - i < AW_VEC ? t.n - i : AW_VEC), b.aligned & 1, x);
-#pragma unroll
-            for (int j = 0; j < AW_VEC; ++j) s = fma((double)x[j], (double)x[j], s);
-        }
+        s += b.g_type == T2_F32 ? chunk_squares<ElemF32, STREAM>(b.g, base, t.n, b.aligned & 1)
+           : b.g_type == T2_BF16 ? chunk_squares<ElemBF16, STREAM>(b.g, base, t.n, b.aligned & 1) : chunk_squares<ElemF16, STREAM>(b.g, base, t.n, b.aligned & 1);
     }
     auto block_sum = [&](double v) {
         for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
@@ -139,7 +170,15 @@ __global__ __launch_bounds__(AW_THREADS) void adamw_norm_kernel(AwNormArgs a) {
     if (threadIdx.x == 0) {
         __hip_atomic_store(a.partial + blockIdx.x, s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");       // the store is at the agent's point of coherence
-        last = __hip_atomic_fetch_add(&a.ctl->ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
+        // the last of its group, and among those the last of all (2048 additions to one address take 20 us)
+        const unsigned group = blockIdx.x % AW_GROUPS, groups = gridDim.x < AW_GROUPS ? gridDim.x : AW_GROUPS;
+        uint32_t *mine = a.ctl->ticket + group * 16, *all = a.ctl->ticket + AW_GROUPS * 16;
+        last = false;
+        if (__hip_atomic_fetch_add(mine, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (gridDim.x - group + AW_GROUPS - 1) / AW_GROUPS - 1) {
+            *mine = 0;                 // for the next launch
+            last = __hip_atomic_fetch_add(all, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == groups - 1;
+            if (last) *all = 0;
+        }
     }
     __syncthreads();
     if (!last) return;
@@ -147,7 +186,6 @@ __global__ __launch_bounds__(AW_THREADS) void adamw_norm_kernel(AwNormArgs a) {
     for (int i = threadIdx.x; i < (int)gridDim.x; i += AW_THREADS) s += __hip_atomic_load(a.partial + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     s = block_sum(s);
     if (threadIdx.x == 0) {
-        a.ctl->ticket = 0;             // for the next launch
         const double norm = a.grad_scale * sqrt(s);
         if (a.norm_out) *a.norm_out = (float)norm;
         else begin_step(a, norm);
@@ -178,8 +216,34 @@ __device__ __forceinline__ uint32_t row_max(uint32_t x) {      // over the 16 la
     return dpp_max<0x140>(x);  // mirrored row
 }
 
-__device__ __forceinline__ float decode8(uint32_t code, float shift) {       // shift: 2^(scale byte - 7)
-    return __builtin_bit_cast(float, ((code & 0x7Fu) << 20) | (code << 24 & 0x80000000u)) * shift;
+// Eight values: two at a time by the converter, times the block's power of two (255: NaN, which the product keeps).  Both are exact.
+__device__ __forceinline__ void decode8(u32v2 codes, int scale, float* x) {
+    typedef float F2 __attribute__((ext_vector_type(2)));
+    const float power = scale == 255 ? __builtin_nanf("") : __builtin_bit_cast(float, (uint32_t)scale << 23);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const F2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes[h], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes[h], true);
+        x[4 * h] = lo[0] * power; x[4 * h + 1] = lo[1] * power; x[4 * h + 2] = hi[0] * power; x[4 * h + 3] = hi[1] * power;
+    }
+}
+
+// The correctly rounded root of every element.  With x normal: from the reciprocal root (one ulp) one correction by the exact residual,
+// a third of what the general function takes; zeros and numbers too small or large for it go
+// through that.
+__device__ __forceinline__ void roots(const float* x, float* r) {
+    float least = x[0], most = x[0];
+#pragma unroll
+    for (int j = 1; j < AW_VEC; ++j) { least = fminf(least, x[j]); most = fmaxf(most, x[j]); }
+    if (__all(least > 1e-30f && most < 1e38f)) {
+#pragma unroll
+        for (int j = 0; j < AW_VEC; ++j) {
+            const float y = __builtin_amdgcn_rsqf(x[j]), s = x[j] * y;
+            r[j] = fmaf(fmaf(-s, s, x[j]), 0.5f * y, s);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < AW_VEC; ++j) r[j] = sqrtf(x[j]);
+    }
 }
 
 // codes of eight elements and the block's scale byte
@@ -219,12 +283,13 @@ template <int BITS>
 __global__ __launch_bounds__(AW_THREADS) void adamw_step_kernel(AwStepArgs a) {
 #pragma clang fp contract(off)       // every product and sum rounded by itself: codes are the definition's, bit for bit
     if (a.ctl->skip) return;
-    const int k = a.chunk_tensor[blockIdx.x];
+    const int chunk = (int)(gridDim.x - 1 - blockIdx.x);      // from the end: what the norm read last is still near
+    const int k = a.chunk_tensor[chunk];
     const AwTensor t = a.tensors[k];
     const AwBound b = a.bound[k];
     if (b.p == nullptr) return;          // a table that was bound for the norm alone
     const float gs = a.ctl->gs, lr_t = a.ctl->lr_t, ic2 = a.ctl->ic2, keep = (float)(1.0 - (double)a.ctl->lr * (double)t.decay);
-    const long long base = (long long)((int)blockIdx.x - t.chunk0) * AW_CHUNK;
+    const long long base = (long long)(chunk - t.chunk0) * AW_CHUNK;
     uint32_t key = t2_mix32(a.seed ^ (AW_STREAM * 0x9E3779B9u));
     key = t2_mix32(key ^ (a.ctl->t * 0x85EBCA6Bu + 0x165667B1u));
     for (int it = 0; it < AW_CHUNK / (AW_THREADS * AW_VEC); ++it) {
@@ -241,23 +306,25 @@ __global__ __launch_bounds__(AW_THREADS) void adamw_step_kernel(AwStepArgs a) {
         } else {
             const u32v2 mc = *(const u32v2*)((const uint8_t*)a.m + at), vc = *(const u32v2*)((const uint8_t*)a.v + at);
             const int sm = a.ms[at / AW_BLOCK], sv = a.vs[at / AW_BLOCK];
-            const float nan = __builtin_nanf("");
+            decode8(mc, sm, m);
+            decode8(vc, sv, v);
 #pragma unroll
-            for (int j = 0; j < AW_VEC; ++j) {
-                const uint32_t cm = (mc[j >> 2] >> (8 * (j & 3))) & 0xFFu, cv = (vc[j >> 2] >> (8 * (j & 3))) & 0xFFu;
-                m[j] = sm == 255 ? nan : __builtin_amdgcn_ldexpf(decode8(cm, 1.f), sm - 7);
-                const float rt = sv == 255 ? nan : __builtin_amdgcn_ldexpf(decode8(cv, 1.f), sv - 7);
-                v[j] = rt * rt;
-            }
+            for (int j = 0; j < AW_VEC; ++j) v[j] = v[j] * v[j];
         }
 #pragma unroll
         for (int j = 0; j < AW_VEC; ++j) {
             const float x = g[j] * gs;
             m[j] = m[j] * a.b1 + x * a.omb1;
             v[j] = v[j] * a.b2 + (x * x) * a.omb2;
-            r[j] = BITS == 32 ? __builtin_amdgcn_sqrtf(v[j]) : sqrtf(v[j]);
-            p[j] = p[j] * keep - lr_t * m[j] * __builtin_amdgcn_rcpf(r[j] * ic2 + a.eps);
         }
+        if constexpr (BITS == 8) {
+            roots(v, r);
+        } else {
+#pragma unroll
+            for (int j = 0; j < AW_VEC; ++j) r[j] = __builtin_amdgcn_sqrtf(v[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < AW_VEC; ++j) p[j] = p[j] * keep - lr_t * m[j] * __builtin_amdgcn_rcpf(r[j] * ic2 + a.eps);
         store8(b.p, b.p_type, i, n, b.aligned & 2, p);
         if (b.c) store8(b.c, b.c_type, i, n, b.aligned & 4, p);
         if constexpr (BITS == 32) {
@@ -341,6 +408,7 @@ extern "C" int t2_adamw_create(t2_ctx* ctx, int n_tensors, const int64_t* sizes,
     t2_adamw* o = new (std::nothrow) t2_adamw();
     if (!o) return fail(T2_ENOMEM, "out of host memory");
     o->device = ctx->device; o->n_tensors = n_tensors; o->bits = state_bits;
+    o->stream = t2_adamw_elements(n_tensors, sizes) >= AW_STREAM_FROM;
     o->b1 = beta1; o->b2 = beta2; o->eps = epsilon; o->seed = seed;
     o->m = m; o->v = v; o->ms = (uint8_t*)m_scale; o->vs = (uint8_t*)v_scale; o->step = (long long*)step;
     int rc;
@@ -398,7 +466,11 @@ static AwNormArgs norm_args(const t2_adamw* o, const void* table, double grad_sc
     a.b1 = o->b1; a.b2 = o->b2; a.grad_scale = grad_scale; a.n_chunks = o->n_chunks;
     return a;
 }
-static dim3 norm_grid(const t2_adamw* o) { return dim3(o->n_chunks < AW_NORM_BLOCKS ? o->n_chunks : AW_NORM_BLOCKS); }
+static void launch_norm(const t2_ctx* ctx, const t2_adamw* o, const AwNormArgs& a) {
+    const dim3 grid(o->n_chunks < AW_NORM_BLOCKS ? o->n_chunks : AW_NORM_BLOCKS), threads(AW_THREADS);
+    if (o->stream) hipLaunchKernelGGL(adamw_norm_kernel<true>, grid, threads, 0, ctx->stream, a);
+    else hipLaunchKernelGGL(adamw_norm_kernel<false>, grid, threads, 0, ctx->stream, a);
+}
 
 extern "C" int t2_adamw_global_norm(t2_ctx* ctx, t2_adamw* o, const void* table, double grad_scale, float* norm_out) {
     T2_TRY(check_call(ctx, o));
@@ -407,7 +479,7 @@ extern "C" int t2_adamw_global_norm(t2_ctx* ctx, t2_adamw* o, const void* table,
     HIP_TRY(dev.err);
     AwNormArgs a = norm_args(o, table, grad_scale);
     a.norm_out = norm_out;
-    hipLaunchKernelGGL(adamw_norm_kernel, norm_grid(o), dim3(AW_THREADS), 0, ctx->stream, a);
+    launch_norm(ctx, o, a);
     HIP_TRY(hipGetLastError());
     return T2_OK;
 }
@@ -420,7 +492,7 @@ extern "C" int t2_adamw_step(t2_ctx* ctx, t2_adamw* o, const void* table, double
     HIP_TRY(dev.err);
     AwNormArgs a = norm_args(o, table, grad_scale);
     a.lr = learning_rate; a.lr_dev = learning_rate_dev; a.clip = clip_norm; a.skip_nonfinite = skip_nonfinite != 0;
-    if (clip_norm > 0.0 || skip_nonfinite) hipLaunchKernelGGL(adamw_norm_kernel, norm_grid(o), dim3(AW_THREADS), 0, ctx->stream, a);
+    if (clip_norm > 0.0 || skip_nonfinite) launch_norm(ctx, o, a);
     else hipLaunchKernelGGL(adamw_begin_kernel, dim3(1), dim3(1), 0, ctx->stream, a);
     AwStepArgs s = {};
     s.tensors = o->tensors; s.chunk_tensor = o->chunk_tensor; s.bound = (const AwBound*)table; s.ctl = o->ctl;

@@ -47,7 +47,7 @@ def _sequence(what: str, t, like: Optional[torch.Tensor] = None) -> torch.Tensor
     if like is None:
         if t.dim() != 3 or t.dtype not in _DTYPES or 0 in t.shape:
             raise ValueError(f"{what} must be a non-empty [B, T, H] tensor of float32, bfloat16 or float16, got {t.dtype} {tuple(t.shape)}")
-    elif t.shape != like.shape or t.dtype != like.dtype or t.device != like.device:
+    elif t.dtype is not like.dtype or t.shape != like.shape or t.get_device() != like.get_device():
         raise ValueError(f"{what} must be {like.dtype} {tuple(like.shape)} on {like.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
     if t.shape[2] > 1 and t.stride(2) != 1:
         raise ValueError(f"the channels of {what} must be contiguous")
@@ -56,7 +56,7 @@ def _sequence(what: str, t, like: Optional[torch.Tensor] = None) -> torch.Tensor
 
 def _output(what: str, t, like: torch.Tensor) -> torch.Tensor:
     if t is None:
-        return torch.empty(like.shape, dtype=like.dtype, device=like.device)
+        return like.new_empty(like.shape)
     _sequence(what, t, like)
     B, T, H = t.shape
     sb, st = t.stride(0), t.stride(1)
@@ -146,8 +146,8 @@ def gated_scan_backward(ctx, tape: ScanTape, dy, dfinal=None):
     device = z.device
     if dfinal is not None:
         dfinal = _rows("dfinal", dfinal, B, H, device)
-    dz, df = (torch.empty(z.shape, dtype=z.dtype, device=device) for _ in range(2))
-    do = None if tape.o is None else torch.empty(z.shape, dtype=z.dtype, device=device)
+    dz, df = z.new_empty(z.shape), z.new_empty(z.shape)
+    do = None if tape.o is None else z.new_empty(z.shape)
     dstate = torch.empty((B, H), dtype=torch.float32, device=device)
     ws, n = _workspace(ctx, B, T, H)
     args = _lib.T2ScanArgs.from_buffer_copy(_lib.SCAN_ARGS.pack(_DTYPES[z.dtype], B, T, H, int(tape.reverse), *_seq(z), *_seq(tape.f), *_seq(tape.o), *_NONE, _ptr(tape.lens), 0, 0,
@@ -163,23 +163,27 @@ def gated_scan_step(ctx, z, f, o, state, active=None, out=None):
     if not (isinstance(z, torch.Tensor) and z.is_cuda and z.dim() == 2 and z.dtype in _DTYPES and z.numel()):
         raise ValueError("z must be a non-empty [B, H] device tensor of float32, bfloat16 or float16")
     B, H = shape = z.shape
-    dtype, device = z.dtype, z.device
-    for what, t in (("z", z), ("f", f), ("o", o), ("out", out)):
-        if t is None and (what == "o" or what == "out"):
-            continue
-        if not isinstance(t, torch.Tensor) or t.shape != shape or t.dtype != dtype or t.device != device or (H > 1 and t.stride(1) != 1):
-            raise ValueError(f"{what} must be a {dtype} {tuple(shape)} tensor on {device} with contiguous rows")
-    if not (isinstance(state, torch.Tensor) and state.device == device and state.dtype == torch.float32 and state.shape == shape
-            and (H == 1 or state.stride(1) == 1)):
-        raise ValueError(f"state must be a float32 [{B}, {H}] tensor on {device} with contiguous rows")
+    dtype, at = z.dtype, z.get_device()
+    zs, fs, os = _row_stride("z", z, shape, dtype, at), _row_stride("f", f, shape, dtype, at), 0 if o is None else _row_stride("o", o, shape, dtype, at)
+    ss = _row_stride("state", state, shape, torch.float32, at)
     if active is not None:
-        if not (isinstance(active, torch.Tensor) and active.device == device and active.dtype == torch.bool and active.shape == shape[:1]):
-            raise ValueError(f"active must be a bool [{B}] tensor on {device}")
+        if not (isinstance(active, torch.Tensor) and active.get_device() == at and active.dtype == torch.bool and active.shape == shape[:1]):
+            raise ValueError(f"active must be a bool [{B}] tensor on {z.device}")
         active = active.contiguous()
     ctx = _context(ctx, z)
-    y = torch.empty(shape, dtype=dtype, device=device) if out is None else out
+    if out is None:
+        y, ys = z.new_empty(shape), H
+    else:
+        y, ys = out, _row_stride("out", out, shape, dtype, at)
     with ctx.ordered():
-        _lib.check(ctx.lib.t2_gated_scan_step(ctx.handle, _DTYPES[dtype], B, H, z.data_ptr(), z.stride(0), f.data_ptr(), f.stride(0), _ptr(o),
-                                              0 if o is None else o.stride(0), state.data_ptr(), state.stride(0), _ptr(active), y.data_ptr(),
-                                              y.stride(0)))
+        _lib.check(ctx.lib.t2_gated_scan_step(ctx.handle, _DTYPES[dtype], B, H, z.data_ptr(), zs, f.data_ptr(), fs, 0 if o is None else o.data_ptr(), os,
+                                              state.data_ptr(), ss, 0 if active is None else active.data_ptr(), y.data_ptr(), ys))
     return y
+
+
+def _row_stride(what: str, t, shape, dtype, at: int) -> int:
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.get_device() == at:
+        row, col = t.stride()
+        if col == 1 or shape[1] == 1:
+            return row
+    raise ValueError(f"{what} must be a {dtype} {tuple(shape)} tensor on cuda:{at} with contiguous rows")
