@@ -24,30 +24,25 @@ __device__ __forceinline__ int row_length(const int64_t* lens, int b, int T) {
 }
 
 // ------------------------------------------------------------------------------------------------
-// A sequence is cut into tiles of C = TG * L steps by 64 channels, one workgroup each.  A thread holds L consecutive steps of 4
-// channels in registers (16 lanes read 64 neighbouring channels of a row: 128 bytes or more), so every input is read once and
-// every output written once.  Inside a tile: each thread composes its steps into h' = A h + B; one wave composes the TG pieces of
-// every channel, finds the state in front of the tile, and hands every thread the state in front of its steps.
+// A sequence is cut into tiles of C = TG * L steps by 4 LANES channels, one workgroup each.  A thread holds L consecutive steps of 4
+// channels in registers (LANES threads read neighbouring channels of a row: 128 bytes and more), so every input is read once and
+// every output written once: the memory rate bounds it, at T = 65536 the forward pass takes 4.6 TB/s (231 us, a copy's 211), and
+// arithmetic takes 40 % of that time.  Inside a tile: each thread composes its steps into h' = A h + B; the first waves compose the
+// TG pieces of every channel, find the state in front of the tile, and hand every thread the state in front of its steps.
 //
 // Across tiles: a tile publishes its composition; the state in front of it is that in front of its group of SCAN_GROUP tiles, taken
 // through the compositions in between in their order; the first tile of a group finds it through the whole group before and
 // publishes it.  The order of every sum is fixed, so results do not depend on timing, and only one hand-over in SCAN_GROUP
-// has to wait for another.  Every word is a value that carries its own validity (all ones: not there yet; a computed NaN is never
+// has to wait for another (16 tiles a group: more registers, 5 to 20 us more at T = 32769 and 65536).  Every word is a value that carries its own validity (all ones: not there yet; a computed NaN is never
 // that pattern), so one relaxed agent-scope access hands it over, without flags or fences.  A workgroup's chain (row and channels) is
 // its index's, its tile is drawn from the chain's counter as it starts: it waits only for workgroups of the chain that have started
-// before it and that wait for none behind them, so every wait ends.  (One counter for all chains: B=2, T=65536, H=1024 draws 8192
-// times from one address; every chain has a counter on a line of its own.)
+// before it and that wait for none behind them, so every wait ends.  Every chain's counter has a line of its own: additions to one
+// address take 10 ns each.
 // ------------------------------------------------------------------------------------------------
-#ifndef SCAN_GROUP
 #define SCAN_GROUP 8
-#endif
-#ifndef SCAN_FW
-#define SCAN_FW 4
-#define SCAN_BW 3
-#endif
 #define SCAN_WAIT_TICKS 200000000ull   /* 2 s of the 100 MHz clock; a wait never comes near it.  Beyond: NaN, not a hang */
 
-struct ScanWs {                        // counters [chains][16] | compositions [ntile][chains][64] | states in front of the groups [ngroup][chains][64]
+struct ScanWs {                        // counters [chains][16] | compositions [ntile][chains][CH] | states in front of the groups [ngroup][chains][CH]
     unsigned* next;
     unsigned long long* piece;
     unsigned* state;
@@ -142,9 +137,9 @@ __device__ __forceinline__ TileIds tile_ids(const t2_scan_args& a, const ScanWs&
 }
 
 // zeros at the positions of the tile that lie behind the row's length
-template <typename E, bool BUF, int L>
+template <typename E, bool BUF, int L, int C>
 __device__ __forceinline__ void zero_rows(const t2_seq& q, int b, int first, int tg, int c, int nc, bool on, int len, int T) {
-    const int rows = T - first;                              // a tile's rows never reach beyond this
+    const int rows = T - first < C ? T - first : C;
     const SeqRows<E, BUF> r(q, b, first, rows, len, false);
 #pragma unroll
     for (int l = 0; l < L; ++l) {
@@ -181,7 +176,7 @@ __global__ __launch_bounds__(LANES* TG, WAVES) void scan_tile_kernel(t2_scan_arg
     const int len = t.len, tg = threadIdx.x / LANES, first = t.tile * C, i0 = tg * L, s0 = first + i0;
     const Channels me = channels<BUF>(t.c0 + (threadIdx.x % LANES) * 4, a.H);
     if (first >= len && t.tile > 0) {
-        zero_rows<E, BUF, L>(a.y, t.b, first, tg, me.c, me.nc, me.mine, len, a.T);
+        zero_rows<E, BUF, L, C>(a.y, t.b, first, tg, me.c, me.nc, me.mine, len, a.T);
         return;
     }
     const int rows = len - first < C ? len - first : C;      // steps that are there: rows - 1 is the tile's last (0: an empty row)
@@ -265,7 +260,7 @@ __global__ __launch_bounds__(LANES* TG, WAVES) void scan_tile_kernel(t2_scan_arg
         }
         out.template store<NT>(i0 + l, me.c, me.nc, i0 + l < rows && me.mine, y[0], y[1], y[2], y[3]);
     }
-    if (rows < C) zero_rows<E, BUF, L>(a.y, t.b, first, tg, me.c, me.nc, me.mine, len, a.T);
+    if (rows < C) zero_rows<E, BUF, L, C>(a.y, t.b, first, tg, me.c, me.nc, me.mine, len, a.T);
 }
 
 // Backward: l_t = the gradient that leaves step t for the state in front of it obeys l_t = a_t (l_{t+1} + g_t), g = dy sigmoid(o), the same
@@ -281,9 +276,9 @@ __global__ __launch_bounds__(LANES* TG, WAVES) void scan_tile_backward_kernel(t2
     const int len = t.len, tg = threadIdx.x / LANES, first = t.tile * C, i0 = tg * L;
     const Channels me = channels<BUF>(t.c0 + (threadIdx.x % LANES) * 4, a.H);
     auto zeros = [&] {
-        zero_rows<E, BUF, L>(a.dz, t.b, first, tg, me.c, me.nc, me.mine, len, a.T);
-        zero_rows<E, BUF, L>(a.df, t.b, first, tg, me.c, me.nc, me.mine, len, a.T);
-        if (GATE) zero_rows<E, BUF, L>(a.do_, t.b, first, tg, me.c, me.nc, me.mine, len, a.T);
+        zero_rows<E, BUF, L, C>(a.dz, t.b, first, tg, me.c, me.nc, me.mine, len, a.T);
+        zero_rows<E, BUF, L, C>(a.df, t.b, first, tg, me.c, me.nc, me.mine, len, a.T);
+        if (GATE) zero_rows<E, BUF, L, C>(a.do_, t.b, first, tg, me.c, me.nc, me.mine, len, a.T);
     };
     if (first >= len && t.tile > 0) { zeros(); return; }
     const int rows = len - first < C ? len - first : C;
@@ -302,21 +297,12 @@ __global__ __launch_bounds__(LANES* TG, WAVES) void scan_tile_backward_kernel(t2
 #pragma unroll
         for (int l = 0; l < L; ++l) zr[l] = z.load(i0 + l, me.c, me.nc, i0 + l < rows);
     }
-    float ga[L][4], gb[L][4], g[L][4], gn[GATE ? L : 1][4];        // gn: g (1 - sigmoid(o)), do but for h
+    float ga[L][4], gb[L][4];
     float A[4] = {1.f, 1.f, 1.f, 1.f}, B[4] = {0.f, 0.f, 0.f, 0.f}, Q[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int l = 0; l < L; ++l)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            gate(E::at(fr[l], j), ga[l][j], gb[l][j]);
-            g[l][j] = E::at(dr[l], j);                             // rows that are not there were read as zeros
-            if (GATE) {
-                float so, sn;
-                gate(E::at(orr[l], j), so, sn);
-                g[l][j] *= so;
-                gn[l][j] = g[l][j] * sn;
-            }
-        }
+        for (int j = 0; j < 4; ++j) gate(E::at(fr[l], j), ga[l][j], gb[l][j]);
     if (rows < C) {
 #pragma unroll
         for (int l = 0; l < L; ++l)
@@ -333,7 +319,10 @@ __global__ __launch_bounds__(LANES* TG, WAVES) void scan_tile_backward_kernel(t2
 #pragma unroll
     for (int l = L - 1; l >= 0; --l)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) Q[j] = ga[l][j] * (Q[j] + g[l][j]);
+        for (int j = 0; j < 4; ++j) {
+            const float dy = E::at(dr[l], j);                      // rows that are not there were read as zeros
+            Q[j] = ga[l][j] * (GATE ? fmaf(dy, sigmoid1(E::at(orr[l], j)), Q[j]) : Q[j] + dy);
+        }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const int k = (threadIdx.x % LANES) * 4 + j;
@@ -382,7 +371,7 @@ __global__ __launch_bounds__(LANES* TG, WAVES) void scan_tile_backward_kernel(t2
     __syncthreads();
     const f32v4 hin = s_h[tg][threadIdx.x % LANES], lin = s_l[tg][threadIdx.x % LANES];
     float h[4] = {hin[0], hin[1], hin[2], hin[3]}, d[4] = {lin[0], lin[1], lin[2], lin[3]};
-    float wf[L][4];                                                // df but for the gradient of h
+    float wf[L][4], g[L][4];                                       // wf: df but for the gradient of h
     const SeqRows<E, BUF> dz(a.dz, t.b, first, rows, len, a.reverse), df(a.df, t.b, first, rows, len, a.reverse);
     const SeqRows<E, BUF> dout(GATE ? a.do_ : a.dz, t.b, first, rows, len, a.reverse);
 #pragma unroll
@@ -393,7 +382,13 @@ __global__ __launch_bounds__(LANES* TG, WAVES) void scan_tile_backward_kernel(t2
             const float z = E::at(zr[l], j);
             wf[l][j] = (h[j] - z) * (ga[l][j] * gb[l][j]);
             h[j] = fmaf(ga[l][j], h[j], gb[l][j] * z);
-            if (GATE) o4[j] = gn[l][j] * h[j];
+            g[l][j] = E::at(dr[l], j);
+            if (GATE) {                                            // again: 2 L registers to keep it cost more (odd: 285 us, 273 so)
+                float so, sn;
+                gate(E::at(orr[l], j), so, sn);
+                g[l][j] *= so;
+                o4[j] = g[l][j] * sn * h[j];
+            }
         }
         if (GATE) dout.template store<NT>(i0 + l, me.c, me.nc, i0 + l < rows && me.mine, o4[0], o4[1], o4[2], o4[3]);
     }
@@ -460,10 +455,10 @@ static constexpr Tile backward_tile[] = {{16, 16, 4}, {16, 32, 8}, {16, 16, 4}, 
 static constexpr int forward_waves[] = {4, 4, 4, 2}, backward_waves[] = {3, 2, 3, 2};     // a SIMD: registers for the tile without spills
 
 static Shape shape_of(bool backward, int B, int T, int H, bool buf) {
-    if (!buf) return NARROW;
     const Tile* tiles = backward ? backward_tile : forward_tile;
-    if (T <= tiles[SHORT].steps()) return SHORT;
+    if (T <= tiles[SHORT].steps() && buf) return SHORT;
     if (T <= tiles[MEDIUM].steps()) return MEDIUM;
+    if (!buf) return NARROW;
     const Tile& w = tiles[WIDE];
     const int64_t blocks = (int64_t)B * ((H + w.channels() - 1) / w.channels()) * ((T + w.steps() - 1) / w.steps());
     return blocks >= 12 * 256 ? WIDE : NARROW;
@@ -471,7 +466,7 @@ static Shape shape_of(bool backward, int B, int T, int H, bool buf) {
 
 static int64_t ws_bytes(int B, int T, int H, Tile t) {
     const int64_t ntile = (T + t.steps() - 1) / t.steps(), chains = (int64_t)B * ((H + t.channels() - 1) / t.channels());
-    if (ntile * chains > 0x7FFFFFFF) return fail(T2_EINVAL, "[%d,%d,%d] is too large for one call", B, T, H);
+    if (ntile * chains > 0xFFFFFFFFLL / (t.lanes * t.tg)) return fail(T2_EINVAL, "[%d,%d,%d] is too large for one call", B, T, H);
     return ntile < 2 ? 0 : chains * 64 + (ntile * 8 + (ntile + SCAN_GROUP - 1) / SCAN_GROUP * 4) * chains * t.channels();
 }
 
@@ -531,7 +526,7 @@ static int launch(t2_ctx* ctx, const t2_scan_args* a) {
 
 template <typename E, bool GATE, bool BACKWARD>
 static int launch_shape(t2_ctx* ctx, const t2_scan_args* a, Shape s, bool buf, bool nt) {
-    if (!buf) return launch<E, GATE, false, false, BACKWARD, NARROW>(ctx, a);
+    if (!buf) return s == MEDIUM ? launch<E, GATE, false, false, BACKWARD, MEDIUM>(ctx, a) : launch<E, GATE, false, false, BACKWARD, NARROW>(ctx, a);
     if (s == SHORT) return launch<E, GATE, true, false, BACKWARD, SHORT>(ctx, a);
     if (s == MEDIUM) return launch<E, GATE, true, false, BACKWARD, MEDIUM>(ctx, a);
     if (s == NARROW) return nt ? launch<E, GATE, true, true, BACKWARD, NARROW>(ctx, a) : launch<E, GATE, true, false, BACKWARD, NARROW>(ctx, a);
