@@ -36,10 +36,11 @@ struct t2_adamw {
     void *m = nullptr, *v = nullptr;
     uint8_t *ms = nullptr, *vs = nullptr;
     long long* step = nullptr;
+    // one allocation: ctl | partial | tensors | chunk_tensor
+    AwCtl* ctl = nullptr;
+    double* partial = nullptr;
     AwTensor* tensors = nullptr;
     int* chunk_tensor = nullptr;
-    double* partial = nullptr;
-    AwCtl* ctl = nullptr;
 };
 
 // ------------------------------------------------------------------------------------------------
@@ -365,34 +366,37 @@ extern "C" int64_t t2_adamw_elements(int n_tensors, const int64_t* sizes) {
 extern "C" int t2_adamw_destroy(t2_adamw* o) {
     if (!o) return T2_OK;
     DeviceScope dev(o->device);
-    if (o->tensors) (void)hipFree(o->tensors);
-    if (o->chunk_tensor) (void)hipFree(o->chunk_tensor);
-    if (o->partial) (void)hipFree(o->partial);
     if (o->ctl) (void)hipFree(o->ctl);
     delete o;
     return T2_OK;
 }
 
 static int build(t2_adamw* o, const int64_t* sizes, const double* decay) {
-    std::vector<AwTensor> ts(o->n_tensors);
-    std::vector<int> map;
+    int64_t chunks = 0;
+    for (int i = 0; i < o->n_tensors; ++i) chunks += (sizes[i] + AW_CHUNK - 1) / AW_CHUNK;
+    const size_t at_partial = sizeof(AwCtl), at_tensors = at_partial + AW_NORM_BLOCKS * sizeof(double),
+                 at_chunks = at_tensors + o->n_tensors * sizeof(AwTensor), bytes = at_chunks + (size_t)chunks * sizeof(int);
+    std::vector<char> image(bytes);                          // the control block and the counters start at zero
+    AwTensor* ts = (AwTensor*)(image.data() + at_tensors);
+    int* map = (int*)(image.data() + at_chunks);
     long long off = 0;
+    int chunk = 0;
     for (int i = 0; i < o->n_tensors; ++i) {
-        ts[i] = {sizes[i], off, (float)decay[i], (int)map.size()};
+        ts[i] = {sizes[i], off, (float)decay[i], chunk};
         off += (sizes[i] + AW_BLOCK - 1) / AW_BLOCK * AW_BLOCK;
-        map.insert(map.end(), (size_t)((sizes[i] + AW_CHUNK - 1) / AW_CHUNK), i);
+        for (int64_t k = 0; k < (sizes[i] + AW_CHUNK - 1) / AW_CHUNK; ++k) map[chunk++] = i;
     }
-    o->n_chunks = (int)map.size();
-    HIP_TRY(hipMalloc(&o->tensors, ts.size() * sizeof(AwTensor)));
-    HIP_TRY(hipMalloc(&o->chunk_tensor, map.size() * sizeof(int)));
-    HIP_TRY(hipMalloc(&o->partial, AW_NORM_BLOCKS * sizeof(double)));
-    HIP_TRY(hipMalloc(&o->ctl, sizeof(AwCtl)));
-    const AwCtl zero = {};
-    HIP_TRY(hipMemcpy(o->tensors, ts.data(), ts.size() * sizeof(AwTensor), hipMemcpyHostToDevice));
-    HIP_TRY(hipMemcpy(o->chunk_tensor, map.data(), map.size() * sizeof(int), hipMemcpyHostToDevice));
-    HIP_TRY(hipMemcpy(o->ctl, &zero, sizeof(AwCtl), hipMemcpyHostToDevice));
+    o->n_chunks = chunk;
+    char* dev = nullptr;
+    HIP_TRY(hipMalloc(&dev, bytes));
+    o->ctl = (AwCtl*)dev;
+    o->partial = (double*)(dev + at_partial);
+    o->tensors = (AwTensor*)(dev + at_tensors);
+    o->chunk_tensor = (int*)(dev + at_chunks);
+    HIP_TRY(hipMemcpy(dev, image.data(), bytes, hipMemcpyHostToDevice));
     return T2_OK;
 }
+static_assert(sizeof(AwCtl) % 8 == 0 && sizeof(AwTensor) % 8 == 0, "parts of the allocation are aligned");
 
 extern "C" int t2_adamw_create(t2_ctx* ctx, int n_tensors, const int64_t* sizes, const double* decay, double beta1, double beta2, double epsilon,
                                int state_bits, uint32_t seed, void* m, void* v, void* m_scale, void* v_scale, int64_t* step, t2_adamw** out) {

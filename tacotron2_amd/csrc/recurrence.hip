@@ -2,6 +2,9 @@
 #include "ctx.h"
 #include "elem.h"
 
+// Sums are fused where fmaf says so and nowhere else: every instance of a kernel rounds alike, whatever the layout it is for.
+#pragma clang fp contract(off)
+
 #define SCAN_LOG2E 1.4426950408889634f
 
 // a = sigmoid(f) and b = 1 - a.  b comes from the same exponential, not from 1 - a: near a = 1 (long memories) that

@@ -242,6 +242,33 @@ def test_captured_step(bits):
         o.close()
 
 
+def test_a_tensor_of_more_than_32_bits():
+    """4.3 G elements with states in 8 bits: blocks at the start, around 2^31 and 2^32 and at the end are held to the restatement."""
+    from tacotron2_amd.training import AdamW
+    n = 2 ** 32 + 700
+    opt = AdamW(None, n, learning_rate=1e-2, beta2=0.99, weight_decay=0.1, state_bits=8, seed=9)
+    p, g = (torch.zeros(n, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    places = [0, 2 ** 31 - 256, 2 ** 32 - 256, 2 ** 32 + 128]
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    for at in places:
+        for t in (p, g):
+            t[at:at + 512] = torch.randn(512, generator=gen, device="cuda").to(torch.bfloat16)
+    raw = lambda t: t.view(torch.uint8).cpu().numpy()  # noqa: E731
+    for step in (1, 2):
+        before = [(raw(opt.m[at:at + 512]), raw(opt.m_scale[at // 128:at // 128 + 4]), raw(opt.v[at:at + 512]), raw(opt.v_scale[at // 128:at // 128 + 4]),
+                   _np(p[at:at + 512])) for at in places]
+        opt.apply_gradients(g, p, clip_norm=0.0)
+        for at, (m8, ms, v8, vs, p0) in zip(places, before):
+            gn = _np(g[at:at + 512])
+            mc, ms, vc, vs, m, r = ref.step8(m8, ms, v8, vs, gn.astype(np.float32), step, 1.0, 0.9, 0.99, 9, at)
+            assert np.array_equal(raw(opt.m[at:at + 512]), mc) and np.array_equal(raw(opt.v[at:at + 512]), vc), (step, at)
+            assert np.array_equal(raw(opt.m_scale[at // 128:at // 128 + 4]), ms) and np.array_equal(raw(opt.v_scale[at // 128:at // 128 + 4]), vs), (step, at)
+            pn, _, _, ep, _, _ = ref.step64(p0, gn, m.astype(np.float64), r.astype(np.float64) ** 2, step, 1.0, 1e-2, 0.9, 0.99, 1e-8, 0.1)
+            _off(_np(p[at:at + 512]), pn, ep, torch.bfloat16, (step, at))
+    assert not p[n - 60:].any() and not p[1000:100000].any()
+    opt.close()
+
+
 def test_refusals():
     from tacotron2_amd._lib import T2Error
     from tacotron2_amd.training import AdamW

@@ -83,6 +83,56 @@ def test_long_sequences(dtype, B, T, H):
         _check(z, f, o, lens, state, dy, dfinal, reverse, dtype)
 
 
+@pytest.mark.parametrize("dtype,B,T,H,reverse", [("bf16", 8, 12300, 512, True), ("f16", 2, 25000, 1001, False), ("f32", 3, 16500, 517, False)])
+def test_large_calls(dtype, B, T, H, reverse):
+    """Enough work for the wide tiles; channels are independent, so some of them are held to the restatement."""
+    from tacotron2_amd import recurrence as R
+    gen = torch.Generator(device="cuda").manual_seed(T)
+    r = lambda *s: torch.randn(s, generator=gen, device="cuda")  # noqa: E731
+    dt = DTYPES[dtype]
+    z, f, o, dy = r(B, T, H).to(dt), (r(B, T, H) * 1.5 + 3).to(dt), r(B, T, H).to(dt), r(B, T, H).to(dt)
+    state, dfinal = r(B, H), r(B, H)
+    lens = torch.tensor([T - 700 * b for b in range(B)], device="cuda")
+    y, final, tape = R.gated_scan(None, z, f, o, lens=lens, state=state, reverse=reverse, tape=True)
+    dz, df, do, dstate = R.gated_scan_backward(None, tape, dy, dfinal)
+    rows, cols = [0, B - 1], sorted({0, 1, 63, 64, 127, 128, 255, 256, 400, H - 5, H - 4, H - 2, H - 1})
+    pick = lambda t: t[rows][..., cols]  # noqa: E731
+    n = lens.cpu().numpy()[rows]
+    x = ref.forward(_np(pick(z)), _np(pick(f)), _np(pick(o)), n, _np(pick(state)), reverse)
+    g = ref.backward(x, _np(pick(dy)), _np(pick(dfinal)), n, reverse)
+    for got, want, bound, what, d in ((y, x["y"], x["ey"], "y", dtype), (final, x["final"], x["efinal"], "final", None), (dz, g["dz"], g["edz"], "dz", dtype),
+                                      (df, g["df"], g["edf"], "df", dtype), (do, g["do"], g["edo"], "do", dtype), (dstate, g["dstate"], g["edstate"], "dstate", None)):
+        _close(pick(got), want, bound, what, d)
+    live = torch.arange(T, device="cuda")[None, :, None] < lens[:, None, None]
+    for t in (y, dz, df, do):
+        assert torch.isfinite(t).all() and not t.masked_select(~live).any()
+
+
+@pytest.mark.parametrize("H", [1, 2, 3])
+def test_narrow_rows(H):
+    for T in (63, 300, 900):
+        z, f, o, state, dy, dfinal = _inputs(3, T, H, "bf16", True, T + H)
+        _check(z, f, o, torch.tensor([T, T // 3, 0], device="cuda"), state, dy, dfinal, True, "bf16")
+
+
+def test_distances_beyond_32_bits():
+    """Rows 2^31 elements apart, and steps further apart than a tile's offsets reach."""
+    from tacotron2_amd import recurrence as R
+    for dtype, stride_b, stride_t, T in (("bf16", 2 ** 31 + 24, 24, 300), ("f32", 24, 2 ** 22, 300), ("f16", 2 ** 23, 2 ** 23, 90)):
+        z, f, o, state, dy, dfinal = _inputs(1 if stride_b == stride_t else 2, T, 24, dtype, True, 6)
+
+        def far(x):
+            size = (x.shape[0] - 1) * stride_b + (T - 1) * stride_t + 24
+            v = torch.empty(size, dtype=x.dtype, device="cuda").as_strided(x.shape, (stride_b, stride_t, 1))
+            v.copy_(x)
+            return v
+        a = R.gated_scan(None, z, f, o, state=state, tape=True)
+        b = R.gated_scan(None, far(z), f, o, state=state, tape=True, out=far(z))
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+        for want, got in zip(R.gated_scan_backward(None, a[2], dy, dfinal), R.gated_scan_backward(None, b[2], far(dy), dfinal)):
+            assert torch.equal(want, got)
+
+
 def test_many_rows():
     z, f, o, state, dy, dfinal = _inputs(300, 131, 70, "bf16", True, 5)
     lens = torch.arange(300, device="cuda", dtype=torch.int32) % 132
