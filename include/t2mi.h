@@ -436,7 +436,7 @@ int t2_griffin_lim(t2_ctx* ctx, const float* spectrogram, int B, int T, int num_
  *    y must not overlap an input or itself.
  *  - lens: dev int64 [B] or NULL (all T).  Values outside [0, T] are taken as 0 and T.  Positions at or behind a row's length are not
  *    read into any result and give y = 0; a length of 0 leaves the state as it was.
- *  - state, final_state: dev fp32 [B][H] or NULL (zeros / not wanted).  They may be the same buffer.
+ *  - state, final_state: dev fp32 [B][H] or NULL (zeros / not wanted); they must not overlap, nor may dfinal and dstate.
  *  - tape: dev fp32 of t2_gated_scan_tape() floats or NULL.  The forward call fills it with the state in front of every
  *    T2_SCAN_SPAN-th step; t2_gated_scan_backward recomputes the rest from there.
  *  - ws: dev buffer of t2_gated_scan_ws() bytes, 16-byte aligned, used by this call only (no content is kept between calls: two captured

@@ -114,29 +114,13 @@ __device__ __forceinline__ float look_back(const ScanWs& w, int i, float first, 
     return h;
 }
 
-struct TileIds { int tile, b, c0, len; unsigned chain, chains; };
-
-template <int CH>
-__device__ __forceinline__ TileIds tile_ids(const t2_scan_args& a, const ScanWs& w, int ntile, bool from_end) {
+// the next tile of a chain (the first where there is but one)
+__device__ __forceinline__ int draw_tile(const ScanWs& w, unsigned chain, int ntile) {
     __shared__ unsigned s_tile;
-    TileIds t;
-    const int ncb = (a.H + CH - 1) / CH;
-    t.chains = (unsigned)a.B * (unsigned)ncb;
-    t.chain = blockIdx.x % t.chains;
-    // Neighbouring channels on one XCD (workgroups go round the eight of them): lines that two tiles share are fetched once.  Long
-    // sequences 4 % faster, rows that start inside a line 6 %.
-    if (t.chains % 8 == 0) t.chain = t.chain % 8 * (t.chains / 8) + t.chain / 8;
-    t.tile = 0;
-    if (ntile > 1) {
-        if (threadIdx.x == 0) s_tile = atomicAdd(w.next + (size_t)t.chain * 16, 1u);
-        __syncthreads();
-        t.tile = __builtin_amdgcn_readfirstlane((int)s_tile);
-    }
-    t.b = (int)(t.chain / (unsigned)ncb);
-    t.c0 = (int)(t.chain - (unsigned)t.b * (unsigned)ncb) * CH;
-    if (from_end) t.tile = ntile - 1 - t.tile;
-    t.len = row_length(a.lens, t.b, a.T);
-    return t;
+    if (ntile < 2) return 0;
+    if (threadIdx.x == 0) s_tile = atomicAdd(w.next + (size_t)chain * 16, 1u);
+    __syncthreads();
+    return __builtin_amdgcn_readfirstlane((int)s_tile);
 }
 
 // zeros at the positions of the tile that lie behind the row's length
@@ -170,221 +154,227 @@ __device__ __forceinline__ int channel_of(int c0, unsigned lane_, int H) {
     return c0 + lane < H ? c0 + lane : -1;
 }
 
-template <typename E, bool GATE, bool BUF, bool NT, int LANES, int TG, int L, int WAVES>
-__global__ __launch_bounds__(LANES* TG, WAVES) void scan_tile_kernel(t2_scan_args a, ScanWs w, int ntile) {
-    constexpr int C = TG * L, CH = 4 * LANES;
-    __shared__ float2 s_piece[TG][CH];
-    __shared__ f32v4 s_in[TG][LANES];
-    const TileIds t = tile_ids<CH>(a, w, ntile, false);
-    const int len = t.len, tg = threadIdx.x / LANES, first = t.tile * C, i0 = tg * L, s0 = first + i0;
-    const Channels me = channels<BUF>(t.c0 + (threadIdx.x % LANES) * 4, a.H);
-    if (first >= len && t.tile > 0) {
-        zero_rows<E, BUF, L, C>(a.y, t.b, first, tg, me.c, me.nc, me.mine, len, a.T);
-        return;
+// A workgroup's place: its row, channels and length, and each thread's channels and first step in a tile.
+template <bool BUF, int LANES, int L>
+struct Place {
+    int b, c0, len, tg, i0;
+    Channels me;
+    __device__ __forceinline__ Place(const t2_scan_args& a, unsigned chain) {
+        const unsigned ncb = (a.H + 4 * LANES - 1) / (4 * LANES);
+        b = (int)(chain / ncb);
+        c0 = (int)(chain - (unsigned)b * ncb) * 4 * LANES;
+        len = row_length(a.lens, b, a.T);
+        tg = threadIdx.x / LANES;
+        i0 = tg * L;
+        me = channels<BUF>(c0 + (threadIdx.x % LANES) * 4, a.H);
     }
-    const int rows = len - first < C ? len - first : C;      // steps that are there: rows - 1 is the tile's last (0: an empty row)
-    typename E::Raw zr[L], fr[L], orr[L];
-    {
-        const SeqRows<E, BUF> f(a.f, t.b, first, rows, len, a.reverse), z(a.z, t.b, first, rows, len, a.reverse);
+    // the steps of the tile from step `first` on that are there (at most C)
+    __device__ __forceinline__ int rows(int first, int C) const { return len - first < C ? len - first : C; }
+    template <typename E>
+    __device__ __forceinline__ void load(typename E::Raw* r, const t2_seq& q, int first, int rows, bool reverse) const {
+        const SeqRows<E, BUF> s(q, b, first, rows, len, reverse);
 #pragma unroll
-        for (int l = 0; l < L; ++l) fr[l] = f.load(i0 + l, me.c, me.nc, i0 + l < rows);
-#pragma unroll
-        for (int l = 0; l < L; ++l) zr[l] = z.load(i0 + l, me.c, me.nc, i0 + l < rows);
+        for (int l = 0; l < L; ++l) r[l] = s.load(i0 + l, me.c, me.nc, i0 + l < rows);
     }
-    if (GATE) {
-        const SeqRows<E, BUF> o(a.o, t.b, first, rows, len, a.reverse);
+    template <typename E, int C>
+    __device__ __forceinline__ void zeros(const t2_seq& q, int first, int T) const { zero_rows<E, BUF, L, C>(q, b, first, tg, me.c, me.nc, me.mine, len, T); }
+};
+
+// Workgroups of neighbouring channels on one XCD (workgroups go round the eight of them): lines that two tiles share are fetched once.
+// Long sequences 4 % faster, rows that start inside a line 6 %.
+__device__ __forceinline__ unsigned chain_of(unsigned index, unsigned chains) {
+    const unsigned c = index % chains;
+    return chains % 8 == 0 ? c % 8 * (chains / 8) + c / 8 : c;
+}
+
+// the composition of all TG pieces of a channel, in the order of the steps or against it
+template <int TG, int CH, bool BACK>
+__device__ __forceinline__ void compose(const float2 (*piece)[CH], unsigned lane, float& A, float& B) {
+    A = 1.f; B = 0.f;
 #pragma unroll
-        for (int l = 0; l < L; ++l) orr[l] = o.load(i0 + l, me.c, me.nc, i0 + l < rows);
+    for (int k = 0; k < TG; ++k) {
+        const float2 p = piece[BACK ? TG - 1 - k : k][lane];
+        B = fmaf(p.x, B, p.y);
+        A *= p.x;
     }
-    float ga[L][4], x[L][4], A[4] = {1.f, 1.f, 1.f, 1.f}, B[4] = {0.f, 0.f, 0.f, 0.f};
+    asm volatile("" ::: "memory");                         // distribute() reads the pieces again: 2 TG registers otherwise
+}
+// v, which enters the tile, taken through the pieces: what enters each of them goes to `in`; returns what leaves
+template <int TG, int CH, bool BACK>
+__device__ __forceinline__ float distribute(const float2 (*piece)[CH], f32v4 (*in)[CH / 4], unsigned lane, float v) {
+#pragma unroll
+    for (int k = 0; k < TG; ++k) {
+        const int i = BACK ? TG - 1 - k : k;
+        const float2 p = piece[i][lane];
+        ((float*)in[i])[lane] = v;
+        v = fmaf(p.x, v, p.y);
+    }
+    return v;
+}
+
+// ---- forward: what a thread does with its L steps of a tile ----
+template <typename E, int L> struct Inputs { typename E::Raw z[L], f[L]; };
+template <int L> struct Steps { float a[L][4], x[L][4]; };          // h' = a h + x
+
+template <typename E, int L>
+__device__ __forceinline__ void steps_of(const Inputs<E, L>& in, int i0, int rows, int C, Steps<L>& s, float2 (&piece)[4]) {
+    float A[4] = {1.f, 1.f, 1.f, 1.f}, B[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int l = 0; l < L; ++l)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             float b;
-            gate(E::at(fr[l], j), ga[l][j], b);
-            x[l][j] = b * E::at(zr[l], j);
+            gate(E::at(in.f[l], j), s.a[l][j], b);
+            s.x[l][j] = b * E::at(in.z[l], j);
         }
     if (rows < C) {                                          // padding: h stays
 #pragma unroll
         for (int l = 0; l < L; ++l)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) if (i0 + l >= rows) { ga[l][j] = 1.f; x[l][j] = 0.f; }
+            for (int j = 0; j < 4; ++j) if (i0 + l >= rows) { s.a[l][j] = 1.f; s.x[l][j] = 0.f; }
     }
 #pragma unroll
     for (int l = 0; l < L; ++l)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            B[j] = fmaf(ga[l][j], B[j], x[l][j]);
-            A[j] *= ga[l][j];
+            B[j] = fmaf(s.a[l][j], B[j], s.x[l][j]);
+            A[j] *= s.a[l][j];
         }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) s_piece[tg][(threadIdx.x % LANES) * 4 + j] = make_float2(A[j], B[j]);
-    __syncthreads();
-    if (threadIdx.x < CH) {
-        const unsigned lane = threadIdx.x;
-        const int cc = channel_of<BUF>(t.c0, lane, a.H);
-        float At = 1.f, Bt = 0.f;
-#pragma unroll
-        for (int i = 0; i < TG; ++i) {
-            const float2 p = s_piece[i][lane];
-            Bt = fmaf(p.x, Bt, p.y);
-            At *= p.x;
-        }
-        const long long line = (long long)t.chains * CH, place = (long long)t.chain * CH, slot = t.tile * line + place;
-        const bool more = first + C < len;                       // a tile behind this one will look back
-        if (more) publish(w.piece + slot + lane, At, Bt);
-        float h = look_back(w, t.tile, a.state && cc >= 0 ? a.state[(long long)t.b * a.H + cc] : 0.f, lane, slot, line, t.tile / SCAN_GROUP * line + place, line);
-        asm volatile("" ::: "memory");                         // the pieces are read again, not kept in 2 TG registers meanwhile
-        if (!more && a.final_state && cc >= 0) a.final_state[(long long)t.b * a.H + cc] = fmaf(At, h, Bt);
-#pragma unroll
-        for (int i = 0; i < TG; ++i) {
-            const float2 p = s_piece[i][lane];
-            ((float*)s_in[i])[lane] = h;
-            h = fmaf(p.x, h, p.y);
-        }
-    }
-    __syncthreads();
-    const f32v4 hin = s_in[tg][threadIdx.x % LANES];
+    for (int j = 0; j < 4; ++j) piece[j] = make_float2(A[j], B[j]);
+}
+
+template <typename E, bool GATE, bool BUF, bool NT, int LANES, int L, int C>
+__device__ __forceinline__ void finish(const t2_scan_args& a, const Place<BUF, LANES, L>& t, int first, int rows, const Steps<L>& s, const typename E::Raw* o, f32v4 hin) {
     float h[4] = {hin[0], hin[1], hin[2], hin[3]};
-    if (a.tape && i0 < rows && s0 % T2_SCAN_SPAN == 0 && me.mine) {
-        float* q = a.tape + ((long long)t.b * ((a.T + T2_SCAN_SPAN - 1) / T2_SCAN_SPAN) + s0 / T2_SCAN_SPAN) * a.H + me.c;
+    const int s0 = first + t.i0;
+    if (a.tape && t.i0 < rows && s0 % T2_SCAN_SPAN == 0 && t.me.mine) {
+        float* q = a.tape + ((long long)t.b * ((a.T + T2_SCAN_SPAN - 1) / T2_SCAN_SPAN) + s0 / T2_SCAN_SPAN) * a.H + t.me.c;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) if (j < me.nc) q[j] = h[j];
+        for (int j = 0; j < 4; ++j) if (j < t.me.nc) q[j] = h[j];
     }
-    const SeqRows<E, BUF> out(a.y, t.b, first, rows, len, a.reverse);
+    const SeqRows<E, BUF> out(a.y, t.b, first, rows, t.len, a.reverse);
 #pragma unroll
     for (int l = 0; l < L; ++l) {
         float y[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            h[j] = fmaf(ga[l][j], h[j], x[l][j]);
-            y[j] = GATE ? h[j] * sigmoid1(E::at(orr[l], j)) : h[j];
+            h[j] = fmaf(s.a[l][j], h[j], s.x[l][j]);
+            y[j] = GATE ? h[j] * sigmoid1(E::at(o[l], j)) : h[j];
         }
-        out.template store<NT>(i0 + l, me.c, me.nc, i0 + l < rows && me.mine, y[0], y[1], y[2], y[3]);
+        out.template store<NT>(t.i0 + l, t.me.c, t.me.nc, t.i0 + l < rows && t.me.mine, y[0], y[1], y[2], y[3]);
     }
-    if (rows < C) zero_rows<E, BUF, L, C>(a.y, t.b, first, tg, me.c, me.nc, me.mine, len, a.T);
+    if (rows < C) t.template zeros<E, C>(a.y, first, a.T);
 }
 
-// Backward: l_t = the gradient that leaves step t for the state in front of it obeys l_t = a_t (l_{t+1} + g_t), g = dy sigmoid(o), the same
-// recurrence from the other end; tiles are drawn from the last to the first and look back at the tiles behind them.  The states inside
-// the tile come from the tape's, which needs no other tile.
 template <typename E, bool GATE, bool BUF, bool NT, int LANES, int TG, int L, int WAVES>
-__global__ __launch_bounds__(LANES* TG, WAVES) void scan_tile_backward_kernel(t2_scan_args a, ScanWs w, int ntile) {
+__global__ __launch_bounds__(LANES* TG, WAVES) void scan_tile_kernel(t2_scan_args a, ScanWs w, int ntile) {
     constexpr int C = TG * L, CH = 4 * LANES;
-    static_assert(C % T2_SCAN_SPAN == 0 && T2_SCAN_SPAN % L == 0, "tiles start where the tape has a state");
-    __shared__ float2 s_fwd[TG][CH], s_bwd[TG][CH];
-    __shared__ f32v4 s_h[TG][LANES], s_l[TG][LANES];
-    const TileIds t = tile_ids<CH>(a, w, ntile, true);
-    const int len = t.len, tg = threadIdx.x / LANES, first = t.tile * C, i0 = tg * L;
-    const Channels me = channels<BUF>(t.c0 + (threadIdx.x % LANES) * 4, a.H);
-    auto zeros = [&] {
-        zero_rows<E, BUF, L, C>(a.dz, t.b, first, tg, me.c, me.nc, me.mine, len, a.T);
-        zero_rows<E, BUF, L, C>(a.df, t.b, first, tg, me.c, me.nc, me.mine, len, a.T);
-        if (GATE) zero_rows<E, BUF, L, C>(a.do_, t.b, first, tg, me.c, me.nc, me.mine, len, a.T);
-    };
-    if (first >= len && t.tile > 0) { zeros(); return; }
-    const int rows = len - first < C ? len - first : C;
-    typename E::Raw zr[L], fr[L], orr[L], dr[L];
-    {
-        const SeqRows<E, BUF> f(a.f, t.b, first, rows, len, a.reverse), z(a.z, t.b, first, rows, len, a.reverse), d(a.dy, t.b, first, rows, len, a.reverse);
+    __shared__ float2 s_piece[TG][CH];
+    __shared__ f32v4 s_in[TG][LANES];
+    const unsigned chains = gridDim.x / (unsigned)ntile, chain = chain_of(blockIdx.x, chains);
+    const Place<BUF, LANES, L> t(a, chain);
+    const int tile = draw_tile(w, chain, ntile), first = tile * C;
+    if (first >= t.len && tile > 0) { t.template zeros<E, C>(a.y, first, a.T); return; }
+    const int rows = t.rows(first, C);
+    Inputs<E, L> in;
+    typename E::Raw o[L];
+    t.template load<E>(in.f, a.f, first, rows, a.reverse);
+    t.template load<E>(in.z, a.z, first, rows, a.reverse);
+    if (GATE) t.template load<E>(o, a.o, first, rows, a.reverse);
+    Steps<L> s;
+    float2 piece[4];
+    steps_of<E, L>(in, t.i0, rows, C, s, piece);
 #pragma unroll
-        for (int l = 0; l < L; ++l) fr[l] = f.load(i0 + l, me.c, me.nc, i0 + l < rows);
-        if (GATE) {
-            const SeqRows<E, BUF> o(a.o, t.b, first, rows, len, a.reverse);
-#pragma unroll
-            for (int l = 0; l < L; ++l) orr[l] = o.load(i0 + l, me.c, me.nc, i0 + l < rows);
-        }
-#pragma unroll
-        for (int l = 0; l < L; ++l) dr[l] = d.load(i0 + l, me.c, me.nc, i0 + l < rows);
-#pragma unroll
-        for (int l = 0; l < L; ++l) zr[l] = z.load(i0 + l, me.c, me.nc, i0 + l < rows);
+    for (int j = 0; j < 4; ++j) s_piece[t.tg][(threadIdx.x % LANES) * 4 + j] = piece[j];
+    __syncthreads();
+    if (threadIdx.x < CH) {
+        const unsigned lane = threadIdx.x;
+        const int cc = channel_of<BUF>(t.c0, lane, a.H);
+        float At, Bt;
+        compose<TG, CH, false>(s_piece, lane, At, Bt);
+        const long long line = (long long)chains * CH, place = (long long)chain * CH, slot = tile * line + place;
+        const bool more = first + C < t.len;                     // a tile behind this one will look back
+        if (more) publish(w.piece + slot + lane, At, Bt);
+        const float h = look_back(w, tile, a.state && cc >= 0 ? a.state[(long long)t.b * a.H + cc] : 0.f, lane, slot, line, tile / SCAN_GROUP * line + place, line);
+        if (!more && a.final_state && cc >= 0) a.final_state[(long long)t.b * a.H + cc] = fmaf(At, h, Bt);
+        distribute<TG, CH, false>(s_piece, s_in, lane, h);
     }
-    float ga[L][4], gb[L][4];
+    __syncthreads();
+    finish<E, GATE, BUF, NT, LANES, L, C>(a, t, first, rows, s, o, s_in[t.tg][threadIdx.x % LANES]);
+}
+
+// ---- backward ----
+// l_t, the gradient that leaves step t for the state in front of it, obeys l_t = a_t (l_{t+1} + g_t), g = dy sigmoid(o): the same
+// recurrence from the other end; tiles are drawn from the last to the first and look back at the tiles behind them.  The states
+// inside a tile come from the tape's, which needs no other tile.
+template <typename E, int L> struct Grads { typename E::Raw z[L], f[L], o[L], d[L]; };
+template <int L> struct BackSteps { float a[L][4], b[L][4]; };
+
+template <typename E, bool GATE, int L>
+__device__ __forceinline__ void back_steps_of(const Grads<E, L>& in, int i0, int rows, int C, BackSteps<L>& s, float2 (&fwd)[4], float2 (&bwd)[4]) {
     float A[4] = {1.f, 1.f, 1.f, 1.f}, B[4] = {0.f, 0.f, 0.f, 0.f}, Q[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int l = 0; l < L; ++l)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) gate(E::at(fr[l], j), ga[l][j], gb[l][j]);
+        for (int j = 0; j < 4; ++j) gate(E::at(in.f[l], j), s.a[l][j], s.b[l][j]);
     if (rows < C) {
 #pragma unroll
         for (int l = 0; l < L; ++l)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) if (i0 + l >= rows) { ga[l][j] = 1.f; gb[l][j] = 0.f; }
+            for (int j = 0; j < 4; ++j) if (i0 + l >= rows) { s.a[l][j] = 1.f; s.b[l][j] = 0.f; }
     }
 #pragma unroll
     for (int l = 0; l < L; ++l)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            B[j] = fmaf(ga[l][j], B[j], gb[l][j] * E::at(zr[l], j));
-            A[j] *= ga[l][j];
+            B[j] = fmaf(s.a[l][j], B[j], s.b[l][j] * E::at(in.z[l], j));
+            A[j] *= s.a[l][j];
         }
 #pragma unroll
     for (int l = L - 1; l >= 0; --l)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const float dy = E::at(dr[l], j);                      // rows that are not there were read as zeros
-            Q[j] = ga[l][j] * (GATE ? fmaf(dy, sigmoid1(E::at(orr[l], j)), Q[j]) : Q[j] + dy);
+            const float dy = E::at(in.d[l], j);                    // rows that are not there were read as zeros
+            Q[j] = s.a[l][j] * (GATE ? fmaf(dy, sigmoid1(E::at(in.o[l], j)), Q[j]) : Q[j] + dy);
         }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const int k = (threadIdx.x % LANES) * 4 + j;
-        s_fwd[tg][k] = make_float2(A[j], B[j]);
-        s_bwd[tg][k] = make_float2(A[j], Q[j]);
+    for (int j = 0; j < 4; ++j) { fwd[j] = make_float2(A[j], B[j]); bwd[j] = make_float2(A[j], Q[j]); }
+}
+
+// the states in front of the pieces, from the tape's
+template <int TG, int L>
+__device__ __forceinline__ float tape_state(const t2_scan_args& a, int b, int first, int rows, int cc, int k) {
+    const int ntape = (a.T + T2_SCAN_SPAN - 1) / T2_SCAN_SPAN;
+    return cc >= 0 && k * T2_SCAN_SPAN < rows ? a.tape[((long long)b * ntape + first / T2_SCAN_SPAN + k) * a.H + cc] : 0.f;
+}
+template <int TG, int L, int CH>
+__device__ __forceinline__ void distribute_states(const t2_scan_args& a, int b, int first, int rows, int cc, const float2 (*piece)[CH], f32v4 (*in)[CH / 4], unsigned lane) {
+    float h = 0.f;
+#pragma unroll
+    for (int i = 0; i < TG; ++i) {
+        if (i * L % T2_SCAN_SPAN == 0) h = tape_state<TG, L>(a, b, first, rows, cc, i * L / T2_SCAN_SPAN);
+        const float2 p = piece[i][lane];
+        ((float*)in[i])[lane] = h;
+        h = fmaf(p.x, h, p.y);
     }
-    __syncthreads();
-    if (threadIdx.x < CH) {                                        // the states, from the tape's
-        const unsigned lane = threadIdx.x;
-        const int cc = channel_of<BUF>(t.c0, lane, a.H), ntape = (a.T + T2_SCAN_SPAN - 1) / T2_SCAN_SPAN;
-        const float* tape = a.tape + ((long long)t.b * ntape + t.tile * (C / T2_SCAN_SPAN)) * a.H + cc;
-        float h = 0.f;
-#pragma unroll
-        for (int i = 0; i < TG; ++i) {
-            const int j = i * L / T2_SCAN_SPAN;
-            if (i * L % T2_SCAN_SPAN == 0) h = cc >= 0 && j * T2_SCAN_SPAN < rows ? tape[(long long)j * a.H] : 0.f;
-            const float2 p = s_fwd[i][lane];
-            ((float*)s_h[i])[lane] = h;
-            h = fmaf(p.x, h, p.y);
-        }
-    }
-    constexpr int SIDE = TG >= 8 ? CH : 0;                         // other waves where there are some: the gradients that enter
-    if (threadIdx.x >= SIDE && threadIdx.x < SIDE + CH) {
-        const unsigned lane = threadIdx.x - SIDE;
-        const int cc = channel_of<BUF>(t.c0, lane, a.H);
-        float At = 1.f, Qt = 0.f;
-#pragma unroll
-        for (int i = TG - 1; i >= 0; --i) {
-            const float2 p = s_bwd[i][lane];
-            Qt = fmaf(p.x, Qt, p.y);
-            At *= p.x;
-        }
-        const int last = len > 0 ? (len - 1) / C : 0, at = last - t.tile;       // the last tile that is not all padding comes first
-        const long long line = (long long)t.chains * CH, place = (long long)t.chain * CH, slot = t.tile * line + place;
-        if (t.tile > 0) publish(w.piece + slot + lane, At, Qt);
-        float l = look_back(w, at, a.dfinal && cc >= 0 ? a.dfinal[(long long)t.b * a.H + cc] : 0.f, lane, slot, -line, at / SCAN_GROUP * line + place, line);
-        asm volatile("" ::: "memory");
-        if (t.tile == 0 && a.dstate && cc >= 0) a.dstate[(long long)t.b * a.H + cc] = fmaf(At, l, Qt);
-#pragma unroll
-        for (int i = TG - 1; i >= 0; --i) {
-            const float2 p = s_bwd[i][lane];
-            ((float*)s_l[i])[lane] = l;
-            l = fmaf(p.x, l, p.y);
-        }
-    }
-    __syncthreads();
-    const f32v4 hin = s_h[tg][threadIdx.x % LANES], lin = s_l[tg][threadIdx.x % LANES];
+}
+
+template <typename E, bool GATE, bool BUF, bool NT, int LANES, int L, int C>
+__device__ __forceinline__ void back_finish(const t2_scan_args& a, const Place<BUF, LANES, L>& t, int first, int rows, const BackSteps<L>& s, const typename E::Raw* zr,
+                                            const typename E::Raw* orr, const typename E::Raw* dr, f32v4 hin, f32v4 lin) {
     float h[4] = {hin[0], hin[1], hin[2], hin[3]}, d[4] = {lin[0], lin[1], lin[2], lin[3]};
     float wf[L][4], g[L][4];                                       // wf: df but for the gradient of h
-    const SeqRows<E, BUF> dz(a.dz, t.b, first, rows, len, a.reverse), df(a.df, t.b, first, rows, len, a.reverse);
-    const SeqRows<E, BUF> dout(GATE ? a.do_ : a.dz, t.b, first, rows, len, a.reverse);
+    const SeqRows<E, BUF> dz(a.dz, t.b, first, rows, t.len, a.reverse), df(a.df, t.b, first, rows, t.len, a.reverse);
+    const SeqRows<E, BUF> dout(GATE ? a.do_ : a.dz, t.b, first, rows, t.len, a.reverse);
 #pragma unroll
     for (int l = 0; l < L; ++l) {
         float o4[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const float z = E::at(zr[l], j);
-            wf[l][j] = (h[j] - z) * (ga[l][j] * gb[l][j]);
-            h[j] = fmaf(ga[l][j], h[j], gb[l][j] * z);
+            wf[l][j] = (h[j] - z) * (s.a[l][j] * s.b[l][j]);
+            h[j] = fmaf(s.a[l][j], h[j], s.b[l][j] * z);
             g[l][j] = E::at(dr[l], j);
             if (GATE) {                                            // again: 2 L registers to keep it cost more (odd: 285 us, 273 so)
                 float so, sn;
@@ -393,7 +383,7 @@ __global__ __launch_bounds__(LANES* TG, WAVES) void scan_tile_backward_kernel(t2
                 o4[j] = g[l][j] * sn * h[j];
             }
         }
-        if (GATE) dout.template store<NT>(i0 + l, me.c, me.nc, i0 + l < rows && me.mine, o4[0], o4[1], o4[2], o4[3]);
+        if (GATE) dout.template store<NT>(t.i0 + l, t.me.c, t.me.nc, t.i0 + l < rows && t.me.mine, o4[0], o4[1], o4[2], o4[3]);
     }
 #pragma unroll
     for (int l = L - 1; l >= 0; --l) {
@@ -401,14 +391,66 @@ __global__ __launch_bounds__(LANES* TG, WAVES) void scan_tile_backward_kernel(t2
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             d[j] += g[l][j];
-            z4[j] = gb[l][j] * d[j];
+            z4[j] = s.b[l][j] * d[j];
             f4[j] = wf[l][j] * d[j];
-            d[j] *= ga[l][j];
+            d[j] *= s.a[l][j];
         }
-        dz.template store<NT>(i0 + l, me.c, me.nc, i0 + l < rows && me.mine, z4[0], z4[1], z4[2], z4[3]);
-        df.template store<NT>(i0 + l, me.c, me.nc, i0 + l < rows && me.mine, f4[0], f4[1], f4[2], f4[3]);
+        dz.template store<NT>(t.i0 + l, t.me.c, t.me.nc, t.i0 + l < rows && t.me.mine, z4[0], z4[1], z4[2], z4[3]);
+        df.template store<NT>(t.i0 + l, t.me.c, t.me.nc, t.i0 + l < rows && t.me.mine, f4[0], f4[1], f4[2], f4[3]);
     }
-    if (rows < C) zeros();
+}
+
+template <typename E, bool GATE, bool BUF, int LANES, int L, int C>
+__device__ __forceinline__ void back_zeros(const t2_scan_args& a, const Place<BUF, LANES, L>& t, int first) {
+    t.template zeros<E, C>(a.dz, first, a.T);
+    t.template zeros<E, C>(a.df, first, a.T);
+    if (GATE) t.template zeros<E, C>(a.do_, first, a.T);
+}
+
+template <typename E, bool GATE, bool BUF, bool NT, int LANES, int TG, int L, int WAVES>
+__global__ __launch_bounds__(LANES* TG, WAVES) void scan_tile_backward_kernel(t2_scan_args a, ScanWs w, int ntile) {
+    constexpr int C = TG * L, CH = 4 * LANES;
+    static_assert(C % T2_SCAN_SPAN == 0 && T2_SCAN_SPAN % L == 0, "tiles start where the tape has a state");
+    static_assert(TG >= 8, "two sets of waves, one for the states and one for the gradients");
+    __shared__ float2 s_fwd[TG][CH], s_bwd[TG][CH];
+    __shared__ f32v4 s_h[TG][LANES], s_l[TG][LANES];
+    const unsigned chains = gridDim.x / (unsigned)ntile, chain = chain_of(blockIdx.x, chains);
+    const Place<BUF, LANES, L> t(a, chain);
+    const int tile = ntile - 1 - draw_tile(w, chain, ntile), first = tile * C;
+    if (first >= t.len && tile > 0) { back_zeros<E, GATE, BUF, LANES, L, C>(a, t, first); return; }
+    const int rows = t.rows(first, C);
+    Grads<E, L> in;
+    t.template load<E>(in.f, a.f, first, rows, a.reverse);
+    if (GATE) t.template load<E>(in.o, a.o, first, rows, a.reverse);
+    t.template load<E>(in.d, a.dy, first, rows, a.reverse);
+    t.template load<E>(in.z, a.z, first, rows, a.reverse);
+    BackSteps<L> s;
+    float2 fwd[4], bwd[4];
+    back_steps_of<E, GATE, L>(in, t.i0, rows, C, s, fwd, bwd);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int k = (threadIdx.x % LANES) * 4 + j;
+        s_fwd[t.tg][k] = fwd[j];
+        s_bwd[t.tg][k] = bwd[j];
+    }
+    __syncthreads();
+    if (threadIdx.x < CH) {
+        distribute_states<TG, L, CH>(a, t.b, first, rows, channel_of<BUF>(t.c0, threadIdx.x, a.H), s_fwd, s_h, threadIdx.x);
+    } else if (threadIdx.x < 2 * CH) {
+        const unsigned lane = threadIdx.x - CH;
+        const int cc = channel_of<BUF>(t.c0, lane, a.H);
+        float At, Qt;
+        compose<TG, CH, true>(s_bwd, lane, At, Qt);
+        const int last = t.len > 0 ? (t.len - 1) / C : 0, at = last - tile;     // the last tile that is not all padding comes first
+        const long long line = (long long)chains * CH, place = (long long)chain * CH, slot = tile * line + place;
+        if (tile > 0) publish(w.piece + slot + lane, At, Qt);
+        const float l = look_back(w, at, a.dfinal && cc >= 0 ? a.dfinal[(long long)t.b * a.H + cc] : 0.f, lane, slot, -line, at / SCAN_GROUP * line + place, line);
+        if (tile == 0 && a.dstate && cc >= 0) a.dstate[(long long)t.b * a.H + cc] = fmaf(At, l, Qt);
+        distribute<TG, CH, true>(s_bwd, s_l, lane, l);
+    }
+    __syncthreads();
+    back_finish<E, GATE, BUF, NT, LANES, L, C>(a, t, first, rows, s, in.z, in.o, in.d, s_h[t.tg][threadIdx.x % LANES], s_l[t.tg][threadIdx.x % LANES]);
+    if (rows < C) back_zeros<E, GATE, BUF, LANES, L, C>(a, t, first);
 }
 
 struct StepArgs {
@@ -447,6 +489,8 @@ extern "C" int64_t t2_gated_scan_tape(int B, int T, int H) {
 // steps (B=32, T=140, H=256 fp32: a call of 14 us, 18.6 with two tiles).  Otherwise 64 channels a tile, which gives more and
 // smaller workgroups, and 128 (256 bytes of a 16-bit row) where there are enough of those for 12 and more on every compute unit:
 // forward 20.4 narrow / 24.0 wide at frames, 251 / 237 at long, 165 / 151 at odd; backward 38.6 / 41.2 at frames, 294 / 277 at odd.
+// (One workgroup for all tiles of a row, the next tile's inputs in flight, needs no workspace either: at frames without lengths 24.5
+// against 25.3 forward and 58 to 64 against 47 backward, elsewhere slower both ways; not taken.)
 struct Tile {
     int lanes, tg, l;
     constexpr int steps() const { return tg * l; }
@@ -493,6 +537,8 @@ static int check_args(const t2_ctx* ctx, const t2_scan_args* a, bool backward) {
     if (!backward && !a->y.ptr) return fail(T2_EINVAL, "y is null");
     if (backward && (!a->dy.ptr || !a->dz.ptr || !a->df.ptr || (a->o.ptr && !a->do_.ptr))) return fail(T2_EINVAL, "dy, dz, df (and do with o) are needed");
     if (backward && !a->tape) return fail(T2_EINVAL, "the tape of the forward call is needed");
+    auto span = [&](const float* p, const float* q) { return p && q && (p < q ? q - p : p - q) < (int64_t)a->B * a->H; };
+    if (span(a->state, a->final_state) || span(a->dfinal, a->dstate)) return fail(T2_EINVAL, "the state before and the state behind overlap");
     const int64_t ws = t2_gated_scan_ws(a->B, a->T, a->H);
     if (ws < 0) return T2_EINVAL;
     if (a->ws_bytes < ws || (ws > 0 && (!a->ws || ((uintptr_t)a->ws & 15)))) return fail(T2_EINVAL, "workspace of %lld bytes, 16-byte aligned, needed", (long long)ws);

@@ -288,7 +288,8 @@ class AdamW:
 
     ``m``, ``v``, ``m_scale``, ``v_scale`` are the live states, tensor i's from ``offsets[i]`` on (``load_state`` sets them).  The step count is
     on the device (``steps()``), so a captured step counts at every replay; capture with a learning rate that is a device scalar
-    where it changes.  ``ctx``: a Context, an Engine, or None for torch's current stream; creating one synchronises, a step does not.
+    where it changes.  Its calls share a workspace: let them follow one another on one stream, or order the streams.  ``ctx``: a Context, an
+    Engine, or None for torch's current stream; creating one synchronises (not while a graph is captured), a step does not.
     Trainer.train_step takes an AdamW of its ``flatten_spec`` in AdamOptimizer's place."""
 
     def __init__(self, ctx, sizes, learning_rate=0.001, beta1=0.9, beta2=0.999, epsilon=1e-8, weight_decay=0.01, state_bits=32, seed=0, device=None):

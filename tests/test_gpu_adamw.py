@@ -102,7 +102,7 @@ def test_steps_of_mixed_tensors(bits, pt, gt, ct):
 
 @pytest.mark.parametrize("bits", [32, 8])
 def test_tensors_that_start_anywhere(bits):
-    for shift, dt in ((1, "f32"), (1, "bf16"), (3, "f16")):
+    for shift, dt in ((1, "f32"), (1, "bf16"), (3, "f16"), (4, "bf16"), (4, "f32")):
         sizes = [130, 8195]
         params, grads, copies = _tensors(sizes, [dt], 3, shift=shift), _tensors(sizes, ["bf16"], 4, shift=shift), _tensors(sizes, ["f16"], 5, shift=1)
         opt, twin = _make(sizes, bits)

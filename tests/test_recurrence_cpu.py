@@ -30,6 +30,10 @@ def test_library_refuses_bad_arguments_before_any_device_work():
         assert fn(None, _args()) == _lib.T2_EINVAL and fn(ctx, None) == _lib.T2_EINVAL
         for kw in bad:
             assert fn(ctx, _args(**kw)) == _lib.T2_EINVAL, kw
+    assert fn is lib.t2_gated_scan_backward
+    both = {"state": 1 << 20, "final_state": (1 << 20) + 4 * 7}                       # of the 8 floats of each, one is shared
+    assert lib.t2_gated_scan(ctx, _args(**both)) == _lib.T2_EINVAL and b"overlap" in lib.t2_last_error()
+    assert lib.t2_gated_scan_backward(ctx, _args(dfinal=1 << 20, dstate=1 << 20)) == _lib.T2_EINVAL and b"overlap" in lib.t2_last_error()
     step = lambda **kw: lib.t2_gated_scan_step(*{**dict(ctx=ctx, dtype=0, B=2, H=4, z=16, zs=4, f=16, fs=4, o=None, os=0, state=16, ss=4, active=None,  # noqa: E731
                                                         y=16, ys=4), **kw}.values())
     for kw in ({"ctx": None}, {"dtype": 5}, {"B": 0}, {"H": 0}, {"z": None}, {"f": None}, {"state": None}, {"y": None}, {"ss": 3}, {"ys": 3}):
