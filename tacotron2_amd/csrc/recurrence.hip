@@ -486,7 +486,9 @@ extern "C" int64_t t2_gated_scan_tape(int B, int T, int H) {
 
 // The tile of a call, by its sizes (kernel times in us; frames: B=32, T=800, H=512 bf16; long: B=2, T=65536, H=1024 bf16; odd: B=2,
 // T=32769, H=1001 fp16).  A sequence that one tile covers needs no workspace, no look back and one launch: tiles of 64 and of 256
-// steps (B=32, T=140, H=256 fp32: a call of 14 us, 18.6 with two tiles).  Otherwise 64 channels a tile, which gives more and
+// steps (B=32, T=140, H=256 fp32: a call of 14 us, 18.6 with two tiles); where 64 channels a workgroup would leave compute units
+// idle, 32 (the same sizes: forward 7.6 -> 6.7, backward 10.0 -> 8.8; B=64, T=250, H=2048 bf16: 62 -> 64, 126 -> 132).  Otherwise
+// 64 channels a tile, which gives more and
 // smaller workgroups, and 128 (256 bytes of a 16-bit row) where there are enough of those for 12 and more on every compute unit:
 // forward 20.4 narrow / 24.0 wide at frames, 251 / 237 at long, 165 / 151 at odd; backward 38.6 / 41.2 at frames, 294 / 277 at odd.
 // (One workgroup for all tiles of a row, the next tile's inputs in flight, needs no workspace either: at frames without lengths 24.5
@@ -496,15 +498,15 @@ struct Tile {
     constexpr int steps() const { return tg * l; }
     constexpr int channels() const { return 4 * lanes; }
 };
-enum Shape { SHORT, MEDIUM, NARROW, WIDE };
-static constexpr Tile forward_tile[] = {{16, 8, 8}, {16, 32, 8}, {16, 16, 8}, {32, 8, 16}};
-static constexpr Tile backward_tile[] = {{16, 16, 4}, {16, 32, 8}, {16, 16, 4}, {32, 8, 8}};
-static constexpr int forward_waves[] = {4, 4, 4, 2}, backward_waves[] = {3, 2, 3, 2};     // a SIMD: registers for the tile without spills
+enum Shape { SHORT, MEDIUM, NARROW, WIDE, FEW };
+static constexpr Tile forward_tile[] = {{16, 8, 8}, {16, 32, 8}, {16, 16, 8}, {32, 8, 16}, {8, 32, 8}};
+static constexpr Tile backward_tile[] = {{16, 16, 4}, {16, 32, 8}, {16, 16, 4}, {32, 8, 8}, {8, 32, 8}};
+static constexpr int forward_waves[] = {4, 4, 4, 2, 4}, backward_waves[] = {3, 2, 3, 2, 2};     // a SIMD: registers for the tile without spills
 
 static Shape shape_of(bool backward, int B, int T, int H, bool buf) {
     const Tile* tiles = backward ? backward_tile : forward_tile;
     if (T <= tiles[SHORT].steps() && buf) return SHORT;
-    if (T <= tiles[MEDIUM].steps()) return MEDIUM;
+    if (T <= tiles[MEDIUM].steps()) return buf && (int64_t)B * ((H + 63) / 64) < 256 ? FEW : MEDIUM;
     if (!buf) return NARROW;
     const Tile& w = tiles[WIDE];
     const int64_t blocks = (int64_t)B * ((H + w.channels() - 1) / w.channels()) * ((T + w.steps() - 1) / w.steps());
@@ -578,6 +580,7 @@ static int launch_shape(t2_ctx* ctx, const t2_scan_args* a, Shape s, bool buf, b
     if (!buf) return s == MEDIUM ? launch<E, GATE, false, false, BACKWARD, MEDIUM>(ctx, a) : launch<E, GATE, false, false, BACKWARD, NARROW>(ctx, a);
     if (s == SHORT) return launch<E, GATE, true, false, BACKWARD, SHORT>(ctx, a);
     if (s == MEDIUM) return launch<E, GATE, true, false, BACKWARD, MEDIUM>(ctx, a);
+    if (s == FEW) return launch<E, GATE, true, false, BACKWARD, FEW>(ctx, a);
     if (s == NARROW) return nt ? launch<E, GATE, true, true, BACKWARD, NARROW>(ctx, a) : launch<E, GATE, true, false, BACKWARD, NARROW>(ctx, a);
     return nt ? launch<E, GATE, true, true, BACKWARD, WIDE>(ctx, a) : launch<E, GATE, true, false, BACKWARD, WIDE>(ctx, a);
 }

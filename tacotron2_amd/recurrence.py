@@ -56,7 +56,7 @@ def _sequence(what: str, t, like: Optional[torch.Tensor] = None) -> torch.Tensor
 
 def _output(what: str, t, like: torch.Tensor) -> torch.Tensor:
     if t is None:
-        return like.new_empty(like.shape)
+        return torch.empty_like(like, memory_format=torch.contiguous_format)
     _sequence(what, t, like)
     B, T, H = t.shape
     sb, st = t.stride(0), t.stride(1)
@@ -79,7 +79,7 @@ def _lengths(lens, B: int, T: int, device) -> Optional[torch.Tensor]:
     if isinstance(lens, torch.Tensor) and lens.is_cuda:
         if tuple(lens.shape) != (B,) or lens.device != device or lens.dtype not in (torch.int64, torch.int32):
             raise ValueError(f"lens must be an int64 or int32 [{B}] tensor on {device}")
-        return lens.to(torch.int64).contiguous()
+        return lens if lens.dtype is torch.int64 and lens.is_contiguous() else lens.to(torch.int64).contiguous()
     host = np.asarray(lens)
     if host.shape != (B,) or host.dtype.kind not in "iu" or (host < 0).any() or (host > T).any():
         raise ValueError(f"lens must be {B} whole numbers from 0 to {T}")
@@ -124,7 +124,7 @@ def gated_scan(ctx, z, f, o=None, lens=None, state=None, reverse: bool = False, 
         state = _rows("state", state, B, H, device)
     lens = _lengths(lens, B, T, device)
     y = _output("out", out, z)
-    final = torch.empty((B, H), dtype=torch.float32, device=device)
+    final = torch.empty_like(state) if state is not None else torch.empty((B, H), dtype=torch.float32, device=device)
     states = torch.empty((B, -(-T // _lib.T2_SCAN_SPAN), H), dtype=torch.float32, device=device) if tape else None
     ws, n = _workspace(ctx, B, T, H)
     args = _lib.T2ScanArgs.from_buffer_copy(_lib.SCAN_ARGS.pack(_DTYPES[z.dtype], B, T, H, 1 if reverse else 0, *_seq(z), *_seq(f), *_seq(o), *_seq(y), _ptr(lens), _ptr(state),
@@ -146,9 +146,9 @@ def gated_scan_backward(ctx, tape: ScanTape, dy, dfinal=None):
     device = z.device
     if dfinal is not None:
         dfinal = _rows("dfinal", dfinal, B, H, device)
-    dz, df = z.new_empty(z.shape), z.new_empty(z.shape)
-    do = None if tape.o is None else z.new_empty(z.shape)
-    dstate = torch.empty((B, H), dtype=torch.float32, device=device)
+    dz, df = _output("dz", None, z), _output("df", None, z)
+    do = None if tape.o is None else _output("do", None, z)
+    dstate = torch.empty_like(dfinal) if dfinal is not None else torch.empty((B, H), dtype=torch.float32, device=device)
     ws, n = _workspace(ctx, B, T, H)
     args = _lib.T2ScanArgs.from_buffer_copy(_lib.SCAN_ARGS.pack(_DTYPES[z.dtype], B, T, H, int(tape.reverse), *_seq(z), *_seq(tape.f), *_seq(tape.o), *_NONE, _ptr(tape.lens), 0, 0,
                                tape.states.data_ptr(), *_seq(dy), *_seq(dz), *_seq(df), *_seq(do), _ptr(dfinal), dstate.data_ptr(), _ptr(ws), n))
@@ -172,7 +172,7 @@ def gated_scan_step(ctx, z, f, o, state, active=None, out=None):
         active = active.contiguous()
     ctx = _context(ctx, z)
     if out is None:
-        y, ys = z.new_empty(shape), H
+        y, ys = torch.empty_like(z, memory_format=torch.contiguous_format), H
     else:
         y, ys = out, _row_stride("out", out, shape, dtype, at)
     with ctx.ordered():
