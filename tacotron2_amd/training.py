@@ -272,6 +272,12 @@ class AdamWBinding:
 
     def __init__(self, table, grads, params, copies):
         self.table, self.grads, self.params, self.copies = table, grads, params, copies
+        self._raw = torch._C._cuda_getCurrentRawStream(table.get_device())
+
+    def _used(self):
+        # on another stream than its own: the table's memory is not given away before that stream is done with it
+        if torch._C._cuda_getCurrentRawStream(self.table.get_device()) != self._raw:
+            self.table.record_stream(torch.cuda.current_stream(self.table.device))
 
 
 class AdamW:
@@ -377,6 +383,7 @@ class AdamW:
     def global_norm(self, grads, grad_scale: float = 1.0) -> torch.Tensor:
         """The norm of grad_scale * all gradients (dev scalar)."""
         b = grads if isinstance(grads, AdamWBinding) else self.bind(grads)
+        b._used()
         ctx = self._context()
         with torch.cuda.device(self.device):
             out = torch.empty(1, dtype=torch.float32, device=self.device)
@@ -405,6 +412,7 @@ class AdamW:
                 raise ValueError(f"a learning rate on the device must be one float32 on {self.device}")
             lr_dev, lr = lr.data_ptr(), 0.0
         ctx = self._context()
+        b._used()
         with ctx.ordered():
             _lib.check(self._lib.t2_adamw_step(ctx.handle, self._h, b.table.data_ptr(), float(lr), lr_dev, float(clip_norm), float(grad_scale),
                                                int(bool(skip_nonfinite))))

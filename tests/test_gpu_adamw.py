@@ -205,6 +205,30 @@ def test_state_round_trip_and_other_streams(bits):
         o.close()
 
 
+def test_a_binding_used_on_another_stream_and_dropped_at_once():
+    opt, _ = _make([3000, 40], 32, seed=3)
+    params = _tensors([3000, 40], ["f32"], 1)
+    g = _tensors([3000, 40], ["f32"], 2)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    for _ in range(4):
+        b = opt.bind(g, params)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(2000000)
+            opt.apply_gradients(b, clip_norm=1.0)
+        at = b.table.data_ptr()
+        n = b.table.numel()
+        del b
+        # the side stream is not done with the table: its memory is not anyone else's yet
+        new = torch.empty(n, dtype=torch.uint8, device="cuda")
+        assert side.query() or new.data_ptr() != at
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+    assert opt.steps() == 4
+    opt.close()
+
+
 @pytest.mark.parametrize("bits", [32, 8])
 def test_captured_step(bits):
     """Replays count and match an eager twin, with eager steps and a learning rate on the device in between; tensors given to a captured
