@@ -362,7 +362,7 @@ extern "C" int64_t t2_adamw_elements(int n_tensors, const int64_t* sizes) {
         if (sizes[i] < 1 || sizes[i] > (1LL << 40)) return fail(T2_EINVAL, "tensor %d has %lld elements", i, (long long)sizes[i]);
         total += (sizes[i] + AW_BLOCK - 1) / AW_BLOCK * AW_BLOCK;
         chunks += (sizes[i] + AW_CHUNK - 1) / AW_CHUNK;
-        if (chunks > 0x7FFFFFFFLL) return fail(T2_EINVAL, "too many elements");
+        if (chunks > 0xFFFFFF) return fail(T2_EINVAL, "too many elements");      // threads of a launch: 32 bits
     }
     return total;
 }

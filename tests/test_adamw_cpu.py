@@ -24,6 +24,7 @@ def test_library_refuses_bad_arguments_before_any_device_work():
         assert create(**kw) == _lib.T2_EINVAL, kw
     assert lib.t2_adamw_elements(2, sizes) == 128 + 256
     assert lib.t2_adamw_elements(1, (C.c_int64 * 1)(1 << 33)) == 1 << 33
+    assert lib.t2_adamw_elements(1, (C.c_int64 * 1)((1 << 37) - 8192)) > 0 and lib.t2_adamw_elements(1, (C.c_int64 * 1)(1 << 37)) < 0    # a launch's threads
     assert lib.t2_adamw_step(None, None, None, 0.0, None, 0.0, 1.0, 0) == _lib.T2_EINVAL and lib.t2_adamw_step(ctx, None, None, 0.0, None, 0.0, 1.0, 0) == _lib.T2_EINVAL
     assert lib.t2_adamw_bind(ctx, None, None, None, None, None, None, None, None) == _lib.T2_EINVAL
     assert lib.t2_adamw_global_norm(ctx, None, None, 1.0, None) == _lib.T2_EINVAL and lib.t2_adamw_table_bytes(None) < 0
