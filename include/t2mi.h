@@ -445,7 +445,9 @@ int t2_griffin_lim(t2_ctx* ctx, const float* spectrogram, int B, int T, int num_
  * t2_gated_scan_backward: dy [B][T][H] of the same type, dfinal dev fp32 [B][H] or NULL (the gradient of final_state) ->
  *     dz, df, do (do where o was given), dstate (dev fp32 [B][H] or NULL); zeros at positions behind a row's length.
  * t2_gated_scan_step: one new position for each row, z, f, o, y [B][H] (stride_b only), state dev fp32 [B][H] with a row stride, updated in place.
- *     active: dev uint8 [B] or NULL; rows where it is 0 keep their state and get y = 0.
+ *     active: dev uint8 [B] or NULL; rows where it is 0 keep their state and get y = 0.  y may be z, f or o itself; otherwise neither it nor
+ *     the state may overlap another tensor.
+ * Outputs that overlap an input or each other are refused where their strides are the same or they start at one place.
  * All three only enqueue; none allocates, so they can be captured. */
 #define T2_F32 0
 #define T2_BF16 1

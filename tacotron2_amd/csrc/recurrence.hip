@@ -29,15 +29,16 @@ __device__ __forceinline__ int row_length(const int64_t* lens, int b, int T) {
 // ------------------------------------------------------------------------------------------------
 // A sequence is cut into tiles of C = TG * L steps by 4 LANES channels, one workgroup each.  A thread holds L consecutive steps of 4
 // channels in registers (LANES threads read neighbouring channels of a row: 128 bytes and more), so every input is read once and
-// every output written once: the memory rate bounds it, at T = 65536 the forward pass takes 4.6 TB/s (231 us, a copy's 211), and
+// every output written once: the memory rate bounds it, at T = 65536 the forward pass takes 4.9 TB/s (220 us, a copy's 211), and
 // arithmetic takes 40 % of that time.  Inside a tile: each thread composes its steps into h' = A h + B; the first waves compose the
 // TG pieces of every channel, find the state in front of the tile, and hand every thread the state in front of its steps.
 //
 // Across tiles: a tile publishes its composition; the state in front of it is that in front of its group of SCAN_GROUP tiles, taken
 // through the compositions in between in their order; the first tile of a group finds it through the whole group before and
 // publishes it.  The order of every sum is fixed, so results do not depend on timing, and only one hand-over in SCAN_GROUP
-// has to wait for another (16 tiles a group: more registers, 5 to 20 us more at T = 32769 and 65536).  Every word is a value that carries its own validity (all ones: not there yet; a computed NaN is never
-// that pattern), so one relaxed agent-scope access hands it over, without flags or fences.  A workgroup's chain (row and channels) is
+// has to wait for another (16 tiles a group: more registers, 5 to 20 us more at T = 32769 and 65536).  Every word is a value that
+// carries its own validity (all ones: not there yet; a computed NaN is never that pattern), so one relaxed agent-scope access hands
+// it over, without flags or fences.  A workgroup's chain (row and channels) is
 // its index's, its tile is drawn from the chain's counter as it starts: it waits only for workgroups of the chain that have started
 // before it and that wait for none behind them, so every wait ends.  Every chain's counter has a line of its own: additions to one
 // address take 10 ns each.
@@ -531,6 +532,26 @@ extern "C" int64_t t2_gated_scan_ws(int B, int T, int H) {
     return most;
 }
 
+// Whether a place of p is one of q (of the same sizes), where their strides are the same or they start at the same place; two
+// patterns of different strides that meet further on are not seen.
+struct Places { const void* ptr; int64_t hi, lo; int n_hi, n_lo; };      // bytes from one to the next, outer and inner axis
+static Places places(const t2_seq& s, int B, int T, int size) {
+    const int64_t b = B > 1 ? s.stride_b * size : 0, t = T > 1 ? s.stride_t * size : 0;
+    return (b < 0 ? -b : b) >= (t < 0 ? -t : t) ? Places{s.ptr, b, t, B, T} : Places{s.ptr, t, b, T, B};
+}
+static bool meet(const Places& p, const Places& q, int64_t row_p, int64_t row_q) {      // row_*: bytes of the channels
+    if (!p.ptr || !q.ptr) return false;
+    const int64_t d = (const char*)q.ptr - (const char*)p.ptr;
+    if (d == 0) return true;
+    if (p.hi != q.hi || p.lo != q.lo || p.n_hi != q.n_hi) return false;
+    for (int64_t i = -1; i <= 1; ++i)
+        for (int64_t j = -1; j <= 1; ++j) {
+            const int64_t kh = p.hi ? d / p.hi + i : 0, r = d - kh * p.hi, kl = p.lo ? r / p.lo + j : 0, e = r - kl * p.lo;
+            if (kh > -p.n_hi && kh < p.n_hi && kl > -p.n_lo && kl < p.n_lo && e < row_p && e > -row_q) return true;
+        }
+    return false;
+}
+
 static int check_args(const t2_ctx* ctx, const t2_scan_args* a, bool backward) {
     if (!ctx || !a) return fail(T2_EINVAL, "null argument");
     if (a->dtype < T2_F32 || a->dtype > T2_F16) return fail(T2_EINVAL, "unknown type %d", a->dtype);
@@ -541,6 +562,16 @@ static int check_args(const t2_ctx* ctx, const t2_scan_args* a, bool backward) {
     if (backward && !a->tape) return fail(T2_EINVAL, "the tape of the forward call is needed");
     auto span = [&](const float* p, const float* q) { return p && q && (p < q ? q - p : p - q) < (int64_t)a->B * a->H; };
     if (span(a->state, a->final_state) || span(a->dfinal, a->dstate)) return fail(T2_EINVAL, "the state before and the state behind overlap");
+    const int size = a->dtype == T2_F32 ? 4 : 2;
+    const t2_seq none = {nullptr, 0, 0}, out[] = {backward ? a->dz : a->y, backward ? a->df : none, backward && a->o.ptr ? a->do_ : none};
+    const t2_seq in[] = {a->z, a->f, a->o, backward ? a->dy : none};
+    for (int i = 0; i < 3; ++i) {
+        if (!out[i].ptr) continue;
+        const Places p = places(out[i], a->B, a->T, size);
+        const int64_t row = (int64_t)a->H * size;
+        for (const t2_seq& q : in) if (meet(p, places(q, a->B, a->T, size), row, row)) return fail(T2_EINVAL, "an output overlaps an input");
+        for (int j = 0; j < i; ++j) if (meet(p, places(out[j], a->B, a->T, size), row, row)) return fail(T2_EINVAL, "two outputs overlap");
+    }
     const int64_t ws = t2_gated_scan_ws(a->B, a->T, a->H);
     if (ws < 0) return T2_EINVAL;
     if (a->ws_bytes < ws || (ws > 0 && (!a->ws || ((uintptr_t)a->ws & 15)))) return fail(T2_EINVAL, "workspace of %lld bytes, 16-byte aligned, needed", (long long)ws);
@@ -623,6 +654,17 @@ extern "C" int t2_gated_scan_step(t2_ctx* ctx, int dtype, int B, int H, const vo
     if (dtype < T2_F32 || dtype > T2_F16) return fail(T2_EINVAL, "unknown type %d", dtype);
     if (!sizes_ok(B, 1, H)) return fail(T2_EINVAL, "bad shape [%d,%d]", B, H);
     if (B > 1 && (state_stride < H || y_stride < H)) return fail(T2_EINVAL, "rows of the state or of y overlap");
+    // y may be z, f or o itself: a thread reads its channel before it writes it
+    const int size = dtype == T2_F32 ? 4 : 2;
+    const void* const in[] = {z, f, o};
+    const int64_t in_stride[] = {z_stride, f_stride, o_stride}, row = (int64_t)H * size;
+    const Places py = places({y, y_stride, 0}, B, 1, size), ps = places({state, state_stride, 0}, B, 1, 4);
+    if (meet(py, ps, row, (int64_t)H * 4)) return fail(T2_EINVAL, "y overlaps the state");
+    for (int i = 0; i < 3; ++i) {
+        const Places q = places({in[i], in_stride[i], 0}, B, 1, size);
+        if (meet(ps, q, (int64_t)H * 4, row)) return fail(T2_EINVAL, "the state overlaps an input");
+        if (!(q.ptr == py.ptr && q.hi == py.hi) && meet(py, q, row, row)) return fail(T2_EINVAL, "y overlaps an input");
+    }
     DeviceScope dev(ctx->device);
     HIP_TRY(dev.err);
     const StepArgs a = {z, f, o, y, state, active, z_stride, f_stride, o_stride, y_stride, state_stride, H};

@@ -150,7 +150,7 @@ _NOTHING = _Nothing()
 
 class StreamContext(Context):
     """A context on a stream of the caller's: the library enqueues where the caller's other work is, and ``ordered`` has nothing
-    to order.  Creating one leaves torch's current device as it was."""
+    to order while that is torch's current stream.  Creating one leaves torch's current device as it was."""
 
     def __init__(self, device: int, stream: torch.cuda.Stream):
         self.lib = _lib.load()
@@ -160,8 +160,10 @@ class StreamContext(Context):
         with torch.cuda.device(self.device):
             _lib.check(self.lib.t2_ctx_create_on_stream(device, C.c_void_p(stream.cuda_stream), C.byref(self.handle)))
 
+        self._raw = stream.cuda_stream
+
     def ordered(self):
-        return _NOTHING
+        return _NOTHING if torch._C._cuda_getCurrentRawStream(self.device.index) == self._raw else super().ordered()
 
 
 _on_stream: Dict[tuple, StreamContext] = {}
@@ -177,7 +179,7 @@ def stream_context(device: Optional[int] = None) -> StreamContext:
     # the bare handle: torch.cuda.current_stream() builds an object, 2 us of a call's 10
     key = (device, torch._C._cuda_getCurrentRawStream(device), threading.get_ident())
     ctx = _on_stream.get(key)
-    if ctx is None:
+    if ctx is None or not ctx.handle:
         ctx = _on_stream[key] = StreamContext(device, torch.cuda.current_stream(device))
     return ctx
 

@@ -159,7 +159,7 @@ def gated_scan_backward(ctx, tape: ScanTape, dy, dfinal=None):
 
 def gated_scan_step(ctx, z, f, o, state, active=None, out=None):
     """One new position for every row: z, f, o (or None) [B, H] -> y [B, H]; ``state`` [B, H] (fp32) is updated in place.  Rows where
-    ``active`` (bool [B] on the device) is False keep their state and get y = 0."""
+    ``active`` (bool [B] on the device) is False keep their state and get y = 0.  ``out`` takes y; it may be z, f or o itself."""
     if not (isinstance(z, torch.Tensor) and z.is_cuda and z.dim() == 2 and z.dtype in _DTYPES and z.numel()):
         raise ValueError("z must be a non-empty [B, H] device tensor of float32, bfloat16 or float16")
     B, H = shape = z.shape

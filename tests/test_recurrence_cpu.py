@@ -34,10 +34,30 @@ def test_library_refuses_bad_arguments_before_any_device_work():
     both = {"state": 1 << 20, "final_state": (1 << 20) + 4 * 7}                       # of the 8 floats of each, one is shared
     assert lib.t2_gated_scan(ctx, _args(**both)) == _lib.T2_EINVAL and b"overlap" in lib.t2_last_error()
     assert lib.t2_gated_scan_backward(ctx, _args(dfinal=1 << 20, dstate=1 << 20)) == _lib.T2_EINVAL and b"overlap" in lib.t2_last_error()
+    at = 1 << 20
+    apart = {"z": (at, 12, 4), "f": (2 * at, 12, 4), "dy": (3 * at, 12, 4), "y": (4 * at, 12, 4), "dz": (5 * at, 12, 4), "df": (6 * at, 12, 4), "ws": None}
+
+    def meets(fn, **kw):
+        assert fn(ctx, _args(**{**apart, **kw})) == _lib.T2_EINVAL, kw
+        return b"overlap" in lib.t2_last_error()
+    # the same place; one channel, one step, one row on; time-major; another layout of the same place
+    for y in ((at, 12, 4), (at + 4, 12, 4), (at - 4 * 4, 12, 4), (at + 4 * 12, 12, 4), (at + 4 * 12 - 12, 12, 4), (at, 100, 8)):
+        assert meets(lib.t2_gated_scan, y=y), y
+    assert meets(lib.t2_gated_scan, z=(at, 4, 8), y=(at + 4 * 8 - 4, 4, 8)) and meets(lib.t2_gated_scan, o=(7 * at, 12, 4), y=(7 * at + 4, 12, 4))
+    for kw in ({"dz": (3 * at, 12, 4)}, {"df": (5 * at + 12, 12, 4)}, {"dz": (2 * at, 12, 4)}, {"o": (7 * at, 12, 4), "do_": (at, 12, 4)},
+               {"o": (7 * at, 12, 4), "do_": (6 * at, 12, 4)}):
+        assert meets(lib.t2_gated_scan_backward, **kw), kw
+    # parts of one [2, 3, 8] tensor: apart, so what is refused is the missing workspace (T = 300) and nothing else
+    slab = {"T": 300, "z": (at, 2400, 8), "y": (at + 16, 2400, 8), "f": (2 * at, 2400, 8)}
+    assert not meets(lib.t2_gated_scan, **slab)
     step = lambda **kw: lib.t2_gated_scan_step(*{**dict(ctx=ctx, dtype=0, B=2, H=4, z=16, zs=4, f=16, fs=4, o=None, os=0, state=16, ss=4, active=None,  # noqa: E731
                                                         y=16, ys=4), **kw}.values())
     for kw in ({"ctx": None}, {"dtype": 5}, {"B": 0}, {"H": 0}, {"z": None}, {"f": None}, {"state": None}, {"y": None}, {"ss": 3}, {"ys": 3}):
         assert step(**kw) == _lib.T2_EINVAL, kw
+    ok = {"z": at, "f": 2 * at, "o": 3 * at, "os": 4, "state": 4 * at, "y": 5 * at}
+    for kw in ({"y": 4 * at}, {"y": 4 * at + 12}, {"y": at + 4}, {"y": 2 * at + 4 * 4}, {"state": at}, {"state": 3 * at + 4}, {"y": at, "ys": 8},
+               {"dtype": 1, "state": at, "ss": 4}):
+        assert step(**{**ok, **kw}) == _lib.T2_EINVAL and b"overlap" in lib.t2_last_error(), kw
     assert lib.t2_gated_scan_tape(2, 65, 3) == 2 * 2 * 3 and lib.t2_gated_scan_tape(0, 1, 1) < 0 and lib.t2_gated_scan_ws(1, 0, 1) < 0
     big = lib.t2_gated_scan_tape(64, 1 << 30, 1 << 12)                               # counts beyond 32 bits
     assert big == 64 * (1 << 24) * (1 << 12)
