@@ -282,8 +282,9 @@ __device__ __forceinline__ u32v2 encode8(const float* x, const uint32_t* word, u
 
 // One pass over parameters, gradients and states; a workgroup takes 8192 neighbouring elements of one tensor, a thread eight at a
 // time, so that one DPP row of 16 lanes finds a block's largest value without shared memory.  Memory bounds it: 27 M elements in
-// fp32 take 140 us (5.5 TB/s), 272 M with 8-bit states, fp32 parameters, bf16 gradients and copies 815 us (5.4 TB/s).  With 16-bit
-// parameters and 8-bit states (10 bytes an element) arithmetic does: 27 M in 59 us, 4.6 TB/s.
+// fp32 take 138 us (5.6 TB/s), 272 M with 8-bit states, fp32 parameters, bf16 gradients and copies 840 us (5.2 TB/s).  With 16-bit
+// parameters and 8-bit states (10 bytes an element) arithmetic does: 27 M in 60 us, 4.6 TB/s; 65 vector instructions an element take
+// three quarters of it.
 template <int BITS>
 __global__ __launch_bounds__(AW_THREADS) void adamw_step_kernel(AwStepArgs a) {
 #pragma clang fp contract(off)       // every product and sum rounded by itself: codes are the definition's, bit for bit

@@ -489,9 +489,9 @@ extern "C" int64_t t2_gated_scan_tape(int B, int T, int H) {
 // T=32769, H=1001 fp16).  A sequence that one tile covers needs no workspace, no look back and one launch: tiles of 64 and of 256
 // steps (B=32, T=140, H=256 fp32: a call of 14 us, 18.6 with two tiles); where 64 channels a workgroup would leave compute units
 // idle, 32 (the same sizes: forward 7.6 -> 6.7, backward 10.0 -> 8.8; B=64, T=250, H=2048 bf16: 62 -> 64, 126 -> 132).  Otherwise
-// 64 channels a tile, which gives more and
-// smaller workgroups, and 128 (256 bytes of a 16-bit row) where there are enough of those for 12 and more on every compute unit:
-// forward 20.4 narrow / 24.0 wide at frames, 251 / 237 at long, 165 / 151 at odd; backward 38.6 / 41.2 at frames, 294 / 277 at odd.
+// 64 channels a tile, which gives more and smaller workgroups, and 128 (256 bytes of a 16-bit row) where there are enough of those
+// for 12 and more on every compute unit: forward 20.4 narrow / 24.0 wide at frames, 241 / 225 at long, 148 / 141 at odd; backward
+// 38.6 / 41.2 at frames, 271 / 262 at odd.  256 channels: 286 at long, 177 and 266 to 274 at odd.
 // (One workgroup for all tiles of a row, the next tile's inputs in flight, needs no workspace either: at frames without lengths 24.5
 // against 25.3 forward and 58 to 64 against 47 backward, elsewhere slower both ways; not taken.)
 struct Tile {
