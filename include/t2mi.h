@@ -486,7 +486,8 @@ int t2_gated_scan_step(t2_ctx* ctx, int dtype, int B, int H, const void* z, int6
  *    (csrc/rng.h) at (seed, stream 20, t, element), a root above zero never to zero.  A block that got a non-finite value stays NaN.
  *  - step: dev int64, the number of steps taken; the device counts, so a captured step counts at every replay.
  *  - t2_adamw_bind writes a table (dev, t2_adamw_table_bytes(), 16-byte aligned) of the tensors' addresses and types on the stream; the
- *    other calls read it.  params may be NULL for a table that only serves the norm; copies (NULL, or NULL entries) get p' in their own type.
+ *    other calls for the same handle read it (a table of another handle has another number of tensors: never give it).  params may be
+ *    NULL for a table that only serves the norm; copies (NULL, or NULL entries) get p' in their own type.
  *  - learning_rate_dev: dev float that replaces learning_rate, or NULL.  skip_nonfinite: a step whose gradient norm is inf or NaN changes
  *    nothing and is not counted.  Without it a NaN reaches the elements that have it (and their blocks of 128 in 8 bits).
  * Calls for one handle must follow one another on the device; the handle's workspace belongs to the call that runs. */

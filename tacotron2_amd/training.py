@@ -267,12 +267,17 @@ class AdamOptimizer:
 
 
 class AdamWBinding:
-    """The tensors of a step, checked once, and their table on the device (``AdamW.bind``).  It stays valid as long as it is kept;
-    it keeps the tensors."""
+    """The tensors of a step, checked once, and their table on the device (``AdamW.bind``).  It stays valid as long as it and its
+    optimizer are kept; it keeps the tensors.  No other optimizer takes it: the kernels read the table by their own optimizer's sizes."""
 
-    def __init__(self, table, grads, params, copies):
+    def __init__(self, handle, table, grads, params, copies):
+        self._handle = handle
         self.table, self.grads, self.params, self.copies = table, grads, params, copies
         self._raw = torch._C._cuda_getCurrentRawStream(table.get_device())
+
+    def _check(self, handle):
+        if handle is None or self._handle is not handle:
+            raise ValueError("this binding is another optimizer's, or its optimizer was closed")
 
     def _used(self):
         # on another stream than its own: the table's memory is not given away before that stream is done with it
@@ -378,11 +383,12 @@ class AdamW:
             table = torch.empty(self._lib.t2_adamw_table_bytes(self._h), dtype=torch.uint8, device=self.device)
             with ctx.ordered():
                 _lib.check(self._lib.t2_adamw_bind(ctx.handle, self._h, *column(grads), *column(params), *column(copies), table.data_ptr()))
-        return AdamWBinding(table, grads, params, copies)
+        return AdamWBinding(self._h, table, grads, params, copies)
 
     def global_norm(self, grads, grad_scale: float = 1.0) -> torch.Tensor:
         """The norm of grad_scale * all gradients (dev scalar)."""
         b = grads if isinstance(grads, AdamWBinding) else self.bind(grads)
+        b._check(self._h)
         b._used()
         ctx = self._context()
         with torch.cuda.device(self.device):
@@ -405,6 +411,7 @@ class AdamW:
             b = self.bind(grads, params, copies)
         if b.params is None:
             raise ValueError("this binding has no params")
+        b._check(self._h)
         lr = self.learning_rate(global_step) if callable(self.learning_rate) else self.learning_rate
         lr_dev = None
         if isinstance(lr, torch.Tensor):

@@ -2,6 +2,7 @@
 import ctypes as C
 
 import numpy as np
+import pytest
 import torch
 
 from tacotron2_amd import _lib
@@ -60,3 +61,27 @@ def test_codes_are_e4m3_and_rounding_is_unbiased():
     x[3] = np.nan
     code, scale = ref.encode(x, np.zeros(128), False)
     assert scale[0] == 255 and np.isnan(ref.decode(code, scale)).all()
+
+
+def test_a_binding_serves_its_own_optimizer_only():
+    """Its table has its optimizer's number of tensors: read by another's it would be left behind its end, or written past a tensor's."""
+    from tacotron2_amd.training import AdamW, AdamWBinding
+
+    def optimizer(sizes):
+        o = AdamW.__new__(AdamW)
+        o.sizes, o.spec, o.learning_rate, o.device, o._ctx, o._lib, o._h = sizes, None, 1e-3, torch.device("cuda", 0), None, None, C.c_void_p(16)
+        return o
+    few, many = optimizer([4]), optimizer([4, 4])
+    b = AdamWBinding.__new__(AdamWBinding)
+    b.table, b.grads, b.params, b.copies, b._raw, b._handle = torch.zeros(48, dtype=torch.uint8), [torch.zeros(4)], [torch.zeros(4)], None, 0, few._h
+    same = optimizer([4])
+    for other in (many, same):
+        with pytest.raises(ValueError):
+            other.apply_gradients(b)
+        with pytest.raises(ValueError):
+            other.global_norm(b)
+    few._h = None                                            # closed
+    with pytest.raises(ValueError):
+        few.apply_gradients(b)
+    for o in (few, many, same):
+        o._h = None                                          # nothing of the library's to give back
