@@ -433,10 +433,9 @@ int t2_griffin_lim(t2_ctx* ctx, const float* spectrogram, int B, int T, int num_
  *     a = sigmoid(f_t)      h_t = a h_{t-1} + (1 - a) z_t      y_t = sigmoid(o_t) h_t   (y_t = h_t where o is NULL)
  * The recurrence is linear in h, so a whole sequence is a scan: it is split over the time axis, not run step by step.
  *  - z, f, o, y: [B][T][H] of one type, channels contiguous, strides in elements (any, 0 for inputs that are broadcast); o may be NULL.
- *    y must not overlap an input or itself.
  *  - lens: dev int64 [B] or NULL (all T).  Values outside [0, T] are taken as 0 and T.  Positions at or behind a row's length are not
  *    read into any result and give y = 0; a length of 0 leaves the state as it was.
- *  - state, final_state: dev fp32 [B][H] or NULL (zeros / not wanted); they must not overlap, nor may dfinal and dstate.
+ *  - state, final_state: dev fp32 [B][H] or NULL (zeros / not wanted).
  *  - tape: dev fp32 of t2_gated_scan_tape() floats or NULL.  The forward call fills it with the state in front of every
  *    T2_SCAN_SPAN-th step; t2_gated_scan_backward recomputes the rest from there.
  *  - ws: dev buffer of t2_gated_scan_ws() bytes, 16-byte aligned, used by this call only (no content is kept between calls: two captured
@@ -447,7 +446,8 @@ int t2_griffin_lim(t2_ctx* ctx, const float* spectrogram, int B, int T, int num_
  * t2_gated_scan_step: one new position for each row, z, f, o, y [B][H] (stride_b only), state dev fp32 [B][H] with a row stride, updated in place.
  *     active: dev uint8 [B] or NULL; rows where it is 0 keep their state and get y = 0.  y may be z, f or o itself; otherwise neither it nor
  *     the state may overlap another tensor.
- * Outputs that overlap an input or each other are refused where their strides are the same or they start at one place.
+ * An output (y, the gradients, final_state, dstate, the tape that is written, ws) that overlaps itself, an input (z, f, o, dy, lens, state, dfinal, the
+ * tape that is read, active) or another output is refused, whatever the strides.
  * All three only enqueue; none allocates, so they can be captured. */
 #define T2_F32 0
 #define T2_BF16 1

@@ -532,24 +532,61 @@ extern "C" int64_t t2_gated_scan_ws(int B, int T, int H) {
     return most;
 }
 
-// Whether a place of p is one of q (of the same sizes), where their strides are the same or they start at the same place; two
-// patterns of different strides that meet further on are not seen.
-struct Places { const void* ptr; int64_t hi, lo; int n_hi, n_lo; };      // bytes from one to the next, outer and inner axis
-static Places places(const t2_seq& s, int B, int T, int size) {
-    const int64_t b = B > 1 ? s.stride_b * size : 0, t = T > 1 ? s.stride_t * size : 0;
-    return (b < 0 ? -b : b) >= (t < 0 ? -t : t) ? Places{s.ptr, b, t, B, T} : Places{s.ptr, t, b, T, B};
+// The bytes of a tensor: rows of `row` bytes, n_hi by n_lo of them, hi and lo bytes from one to the next (hi >= lo, from the lowest on).
+struct Places { int64_t at, hi, lo, n_hi, n_lo, row; };
+static Places places(const void* ptr, int64_t stride_b, int64_t stride_t, int64_t B, int64_t T, int64_t row) {      // strides in bytes
+    if (B == 1) stride_b = 0;
+    if (T == 1) stride_t = 0;
+    int64_t at = (int64_t)ptr;
+    if (stride_b < 0) { at += stride_b * (B - 1); stride_b = -stride_b; }
+    if (stride_t < 0) { at += stride_t * (T - 1); stride_t = -stride_t; }
+    if (stride_b == 0) B = 1;                              // all in one place
+    if (stride_t == 0) T = 1;
+    return stride_b >= stride_t ? Places{at, stride_b, stride_t, B, T, row} : Places{at, stride_t, stride_b, T, B, row};
 }
-static bool meet(const Places& p, const Places& q, int64_t row_p, int64_t row_q) {      // row_*: bytes of the channels
-    if (!p.ptr || !q.ptr) return false;
-    const int64_t d = (const char*)q.ptr - (const char*)p.ptr;
-    if (d == 0) return true;
-    if (p.hi != q.hi || p.lo != q.lo || p.n_hi != q.n_hi) return false;
-    for (int64_t i = -1; i <= 1; ++i)
-        for (int64_t j = -1; j <= 1; ++j) {
-            const int64_t kh = p.hi ? d / p.hi + i : 0, r = d - kh * p.hi, kl = p.lo ? r / p.lo + j : 0, e = r - kl * p.lo;
-            if (kh > -p.n_hi && kh < p.n_hi && kl > -p.n_lo && kl < p.n_lo && e < row_p && e > -row_q) return true;
-        }
+static Places block(const void* ptr, int64_t bytes) { return {(int64_t)ptr, 0, 0, 1, 1, bytes}; }
+static int64_t length(const Places& p) { return p.hi * (p.n_hi - 1) + p.lo * (p.n_lo - 1) + p.row; }
+// every run of n_lo rows ends before the next begins
+static bool nested(const Places& p, int64_t row) { return p.n_hi == 1 || p.hi >= p.lo * (p.n_lo - 1) + row; }
+
+// Whether a row of q meets the n bytes from x on: i hi + j lo lies in [from, to].  One run is looked up by a division; there are more than a
+// few runs to look at only where those of q reach into each other (inputs that are windows of one signal).
+static bool meets_block(int64_t x, int64_t n, const Places& q) {
+    const int64_t from = x - q.row + 1 - q.at, to = x + n - 1 - q.at, run = q.lo * (q.n_lo - 1);
+    if (to < 0) return false;
+    const int64_t first = q.hi && from > run ? (from - run + q.hi - 1) / q.hi : 0, last = q.hi && to / q.hi < q.n_hi - 1 ? to / q.hi : q.n_hi - 1;
+    for (int64_t i = first; i <= last; ++i) {
+        const int64_t a = from - i * q.hi, j = a <= 0 ? 0 : q.lo ? (a + q.lo - 1) / q.lo : q.n_lo;
+        if (j < q.n_lo && j * q.lo <= to - i * q.hi) return true;
+    }
     return false;
+}
+static bool meet(const Places& p, const Places& q) {
+    if (!p.at || !q.at || q.at >= p.at + length(p) || p.at >= q.at + length(q)) return false;
+    if (p.hi == q.hi && p.lo == q.lo && p.n_hi == q.n_hi && p.n_lo == q.n_lo && nested(p, p.row > q.row ? p.row : q.row)) {
+        // the same pattern: two rows kh and kl apart, one of the nine next to the quotients
+        const int64_t d = q.at - p.at;
+        for (int64_t i = -1; i <= 1; ++i)
+            for (int64_t j = -1; j <= 1; ++j) {
+                const int64_t kh = p.hi ? d / p.hi + i : 0, r = d - kh * p.hi, kl = p.lo ? r / p.lo + j : 0, e = r - kl * p.lo;
+                if (kh > -p.n_hi && kh < p.n_hi && kl > -p.n_lo && kl < p.n_lo && e < p.row && e > -q.row) return true;
+            }
+        return false;
+    }
+    const bool fewer = p.n_hi * p.n_lo <= q.n_hi * q.n_lo;         // row by row of the one that has fewer
+    const Places &s = fewer ? p : q, &m = fewer ? q : p;
+    for (int64_t i = 0; i < s.n_hi; ++i)
+        for (int64_t j = 0; j < s.n_lo; ++j)
+            if (meets_block(s.at + i * s.hi + j * s.lo, s.row, m)) return true;
+    return false;
+}
+// a tensor whose rows go round memory more than once is none
+static bool reaches(const t2_seq& s, int B, int T) {
+    const __int128 b = B > 1 ? s.stride_b : 0, t = T > 1 ? s.stride_t : 0;
+    return (b < 0 ? -b : b) * (B - 1) + (t < 0 ? -t : t) * (T - 1) < (1LL << 52);
+}
+static bool meets_itself(const t2_seq& s, const Places& p, int B, int T) {
+    return (B > 1 && s.stride_b == 0) || (T > 1 && s.stride_t == 0) || (p.n_lo > 1 && p.lo < p.row) || !nested(p, p.row);
 }
 
 static int check_args(const t2_ctx* ctx, const t2_scan_args* a, bool backward) {
@@ -560,20 +597,37 @@ static int check_args(const t2_ctx* ctx, const t2_scan_args* a, bool backward) {
     if (!backward && !a->y.ptr) return fail(T2_EINVAL, "y is null");
     if (backward && (!a->dy.ptr || !a->dz.ptr || !a->df.ptr || (a->o.ptr && !a->do_.ptr))) return fail(T2_EINVAL, "dy, dz, df (and do with o) are needed");
     if (backward && !a->tape) return fail(T2_EINVAL, "the tape of the forward call is needed");
-    auto span = [&](const float* p, const float* q) { return p && q && (p < q ? q - p : p - q) < (int64_t)a->B * a->H; };
-    if (span(a->state, a->final_state) || span(a->dfinal, a->dstate)) return fail(T2_EINVAL, "the state before and the state behind overlap");
-    const int size = a->dtype == T2_F32 ? 4 : 2;
-    const t2_seq none = {nullptr, 0, 0}, out[] = {backward ? a->dz : a->y, backward ? a->df : none, backward && a->o.ptr ? a->do_ : none};
-    const t2_seq in[] = {a->z, a->f, a->o, backward ? a->dy : none};
-    for (int i = 0; i < 3; ++i) {
-        if (!out[i].ptr) continue;
-        const Places p = places(out[i], a->B, a->T, size);
-        const int64_t row = (int64_t)a->H * size;
-        for (const t2_seq& q : in) if (meet(p, places(q, a->B, a->T, size), row, row)) return fail(T2_EINVAL, "an output overlaps an input");
-        for (int j = 0; j < i; ++j) if (meet(p, places(out[j], a->B, a->T, size), row, row)) return fail(T2_EINVAL, "two outputs overlap");
-    }
     const int64_t ws = t2_gated_scan_ws(a->B, a->T, a->H);
     if (ws < 0) return T2_EINVAL;
+    // what is written against what is read and what else is written; the tape is written by the forward call and read by the other
+    const int64_t size = a->dtype == T2_F32 ? 4 : 2, row = a->H * size, states = (int64_t)a->B * a->H * 4;
+    const t2_seq none = {nullptr, 0, 0}, seq_in[] = {a->z, a->f, a->o, backward ? a->dy : none};
+    const t2_seq seq_out[] = {backward ? a->dz : a->y, backward ? a->df : none, backward && a->o.ptr ? a->do_ : none};
+    Places in[7], out[6];
+    int n_in = 0, n_out = 0;
+    auto seq = [&](const t2_seq& s) { return places(s.ptr, s.stride_b * size, s.stride_t * size, a->B, a->T, row); };
+    for (const t2_seq& s : seq_in) {
+        if (!s.ptr) continue;
+        if (!reaches(s, a->B, a->T)) return fail(T2_EINVAL, "strides of %lld and %lld elements", (long long)s.stride_b, (long long)s.stride_t);
+        in[n_in++] = seq(s);
+    }
+    for (const t2_seq& s : seq_out) {
+        if (!s.ptr) continue;
+        if (!reaches(s, a->B, a->T)) return fail(T2_EINVAL, "strides of %lld and %lld elements", (long long)s.stride_b, (long long)s.stride_t);
+        out[n_out++] = seq(s);
+        if (meets_itself(s, out[n_out - 1], a->B, a->T)) return fail(T2_EINVAL, "the elements of an output overlap (strides %lld, %lld)", (long long)s.stride_b, (long long)s.stride_t);
+    }
+    const Places tape = block(a->tape, t2_gated_scan_tape(a->B, a->T, a->H) * 4);
+    in[n_in++] = block(a->lens, (int64_t)a->B * 8);
+    in[n_in++] = block(backward ? a->dfinal : a->state, states);
+    if (backward) in[n_in++] = tape;
+    else out[n_out++] = tape;
+    out[n_out++] = block(backward ? a->dstate : a->final_state, states);
+    if (ws > 0) out[n_out++] = block(a->ws, ws);
+    for (int i = 0; i < n_out; ++i) {
+        for (int j = 0; j < n_in; ++j) if (meet(out[i], in[j])) return fail(T2_EINVAL, "an output overlaps an input");
+        for (int j = 0; j < i; ++j) if (meet(out[i], out[j])) return fail(T2_EINVAL, "two outputs overlap");
+    }
     if (a->ws_bytes < ws || (ws > 0 && (!a->ws || ((uintptr_t)a->ws & 15)))) return fail(T2_EINVAL, "workspace of %lld bytes, 16-byte aligned, needed", (long long)ws);
     return T2_OK;
 }
@@ -655,15 +709,17 @@ extern "C" int t2_gated_scan_step(t2_ctx* ctx, int dtype, int B, int H, const vo
     if (!sizes_ok(B, 1, H)) return fail(T2_EINVAL, "bad shape [%d,%d]", B, H);
     if (B > 1 && (state_stride < H || y_stride < H)) return fail(T2_EINVAL, "rows of the state or of y overlap");
     // y may be z, f or o itself: a thread reads its channel before it writes it
-    const int size = dtype == T2_F32 ? 4 : 2;
+    const int64_t size = dtype == T2_F32 ? 4 : 2, row = H * size, in_stride[] = {z_stride, f_stride, o_stride};
     const void* const in[] = {z, f, o};
-    const int64_t in_stride[] = {z_stride, f_stride, o_stride}, row = (int64_t)H * size;
-    const Places py = places({y, y_stride, 0}, B, 1, size), ps = places({state, state_stride, 0}, B, 1, 4);
-    if (meet(py, ps, row, (int64_t)H * 4)) return fail(T2_EINVAL, "y overlaps the state");
+    for (int64_t s : {z_stride, f_stride, o_stride, state_stride, y_stride})
+        if (!reaches({nullptr, s, 0}, B, 1)) return fail(T2_EINVAL, "a stride of %lld elements", (long long)s);
+    const Places py = places(y, y_stride * size, 0, B, 1, row), ps = places(state, state_stride * 4, 0, B, 1, (int64_t)H * 4), pa = block(active, B);
+    if (meet(py, ps)) return fail(T2_EINVAL, "y overlaps the state");
+    if (meet(py, pa) || meet(ps, pa)) return fail(T2_EINVAL, "an output overlaps active");
     for (int i = 0; i < 3; ++i) {
-        const Places q = places({in[i], in_stride[i], 0}, B, 1, size);
-        if (meet(ps, q, (int64_t)H * 4, row)) return fail(T2_EINVAL, "the state overlaps an input");
-        if (!(q.ptr == py.ptr && q.hi == py.hi) && meet(py, q, row, row)) return fail(T2_EINVAL, "y overlaps an input");
+        const Places q = places(in[i], in_stride[i] * size, 0, B, 1, row);
+        if (meet(ps, q)) return fail(T2_EINVAL, "the state overlaps an input");
+        if (!(q.at == py.at && q.hi == py.hi) && meet(py, q)) return fail(T2_EINVAL, "y overlaps an input");
     }
     DeviceScope dev(ctx->device);
     HIP_TRY(dev.err);

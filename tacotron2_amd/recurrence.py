@@ -112,7 +112,8 @@ def gated_scan(ctx, z, f, o=None, lens=None, state=None, reverse: bool = False, 
     Any batch and time strides (time-major views, slices of a projection, broadcast inputs), contiguous channels.  ``lens`` [B]: row b
     has positions 0 .. lens[b] - 1; the others give y = 0 and do not touch the state.  Host lengths outside [0, T] raise, device
     lengths are taken as the nearest.  ``reverse`` runs every row from its last position to its first.  ``state``: the state in
-    front of the first step (fp32 [B, H], default zeros).  ``out`` takes y (a [B, T, H] view; it must not overlap an input)."""
+    front of the first step (fp32 [B, H], default zeros).  ``out`` takes y (a [B, T, H] view; it must not overlap z, f, o or lens; a state that
+    lies in it, such as the last row of the chunk before, is copied first)."""
     _sequence("z", z)
     B, T, H = z.shape
     _sequence("f", f, z)
@@ -124,6 +125,10 @@ def gated_scan(ctx, z, f, o=None, lens=None, state=None, reverse: bool = False, 
         state = _rows("state", state, B, H, device)
     lens = _lengths(lens, B, T, device)
     y = _output("out", out, z)
+    if state is not None and out is not None:
+        begin, end = y.data_ptr(), y.data_ptr() + ((B - 1) * y.stride(0) + (T - 1) * y.stride(1) + H) * y.element_size()
+        if state.data_ptr() < end and state.data_ptr() + 4 * B * H > begin:
+            state = state.clone()
     final = torch.empty_like(state) if state is not None else torch.empty((B, H), dtype=torch.float32, device=device)
     states = torch.empty((B, -(-T // _lib.T2_SCAN_SPAN), H), dtype=torch.float32, device=device) if tape else None
     ws, n = _workspace(ctx, B, T, H)

@@ -99,3 +99,74 @@ def test_restatement_against_a_loop_and_differences(reverse):
             up[i][at] += 1e-5
             down[i][at] -= 1e-5
             assert abs((loss(*up) - loss(*down)) / 2e-5 - g[k][at]) < 1e-8
+
+
+def test_overlaps_of_every_kind_are_refused_before_any_device_work():
+    """What a tile writes, another tile may still have to read: the states, the tape, the lengths and the workspace count like z, f and o."""
+    lib = _lib.load()
+    ctx = C.create_string_buffer(64)
+    at, T, H, B = 1 << 20, 300, 4, 2
+    place = lambda k: (k * at, T * H, H)  # noqa: E731
+    base = {"B": B, "T": T, "H": H, "z": place(1), "f": place(2), "y": place(3), "dy": place(4), "dz": place(5), "df": place(6), "tape": 7 * at, "state": 8 * at,
+            "final_state": 9 * at, "dfinal": 10 * at, "dstate": 11 * at, "lens": 12 * at, "ws": 13 * at, "ws_bytes": 0}
+
+    def refused(fn, **kw):
+        assert fn(ctx, _args(**{**base, **kw})) == _lib.T2_EINVAL
+        return lib.t2_last_error()
+    for fn in (lib.t2_gated_scan, lib.t2_gated_scan_backward):
+        assert b"workspace" in refused(fn)                                          # apart: only the workspace is too small
+    last = 3 * at + (T * H - H) * 4                                                 # the last row of y's first sequence
+    n_tape = lib.t2_gated_scan_tape(B, T, H) * 4
+    for kw in ({"state": last}, {"state": last + 12}, {"state": last - B * H * 4 + 4}, {"final_state": last}, {"lens": last - 8}, {"lens": 9 * at + 28},
+               {"tape": last}, {"tape": 3 * at - n_tape + 4}, {"tape": 8 * at + 28}, {"tape": 12 * at - n_tape + 4}, {"ws": last - 4}, {"ws": 7 * at},
+               {"final_state": 8 * at}, {"y": (3 * at, 0, H)}, {"y": (3 * at, T * H, 0)}, {"y": (3 * at, T * H, H - 1)}, {"y": (3 * at, T * H - 1, H)},
+               {"y": (3 * at, H - 1, 2 * H)}):
+        assert b"overlap" in refused(lib.t2_gated_scan, **kw), kw
+    for kw in ({"dz": (7 * at + n_tape - 4, T * H, H)}, {"df": (10 * at + 28, T * H, H)}, {"dz": (12 * at + 15, T * H, H)}, {"dstate": 7 * at}, {"dstate": 10 * at},
+               {"dstate": 6 * at + 4}, {"dstate": 12 * at}, {"ws": 10 * at}, {"ws": 6 * at}, {"dz": (5 * at, T * H, 0)}):
+        assert b"overlap" in refused(lib.t2_gated_scan_backward, **kw), kw
+    # states that lie in front of the first and behind the last element are apart
+    for kw in ({"state": 3 * at - B * H * 4}, {"state": 3 * at + B * T * H * 4}, {"lens": 3 * at - B * 8}, {"tape": 3 * at + B * T * H * 4}):
+        assert b"workspace" in refused(lib.t2_gated_scan, **kw), kw
+    # strides that no memory holds
+    assert b"strides" in refused(lib.t2_gated_scan, z=(at, 1 << 62, H)) and b"strides" in refused(lib.t2_gated_scan, y=(at, H, -(1 << 62)))
+    step = lambda **kw: lib.t2_gated_scan_step(*{**dict(ctx=ctx, dtype=0, B=2, H=4, z=at, zs=4, f=2 * at, fs=4, o=None, os=0, state=4 * at, ss=4, active=6 * at,  # noqa: E731
+                                                        y=5 * at, ys=4), **kw}.values())
+    for kw in ({"active": 4 * at + 31}, {"active": 5 * at}, {"zs": 5, "z": 4 * at + 8}, {"zs": 0, "z": 5 * at + 16}, {"zs": -4, "z": 5 * at + 40}):
+        assert step(**kw) == _lib.T2_EINVAL and b"overlap" in lib.t2_last_error(), kw
+
+
+def test_overlaps_of_different_strides_are_found_exactly():
+    """Against the sets of bytes themselves: broadcast, reversed, windowed and interleaved inputs around an output in one buffer."""
+    lib = _lib.load()
+    ctx = C.create_string_buffer(64)
+    rng = np.random.default_rng(12)
+    T, far, seen = 257, 1 << 30, [0, 0]
+    for _ in range(400):
+        B, H = int(rng.integers(1, 4)), int(rng.integers(1, 6))
+        if rng.random() < 0.5:
+            st = H + int(rng.integers(0, 9))
+            sb = (T - 1) * st + H + int(rng.integers(0, 40))
+        else:
+            sb = H + int(rng.integers(0, 9))
+            st = (B - 1) * sb + H + int(rng.integers(0, 20))
+        zb, zt = (int(rng.choice([0, sb, -sb, st, 1, H, 3 * H, T * H])), int(rng.choice([0, st, -st, sb, 1, H, 2 * H, B * H])))
+        if B == 1:
+            zb = int(rng.choice([0, 7, -7]))
+
+        def covered(ptr, b, t, row):
+            rows = ptr + 4 * (np.arange(B)[:, None] * b + np.arange(T)[None, :] * t)
+            return np.unique(rows[..., None] + np.arange(row))
+        span = 4 * ((B - 1) * sb + (T - 1) * st + H)
+        y = far
+        z = far + 4 * int(rng.integers(-200, span // 4 + 200)) + 4 * (max(0, -zb) * (B - 1) + max(0, -zt) * (T - 1))
+        state = far + 4 * int(rng.integers(-40, span // 4 + 40))
+        ours = covered(y, sb, st, 4 * H)
+        for kw, theirs in (({"z": (z, zb, zt)}, covered(z, zb, zt, 4 * H)), ({"state": state}, np.arange(state, state + 4 * B * H))):
+            args = _args(**{"B": B, "T": T, "H": H, "z": (far // 2, T * H, H), "f": (far // 4, T * H, H), "y": (y, sb, st), "tape": None, **kw})
+            assert lib.t2_gated_scan(ctx, args) == _lib.T2_EINVAL
+            want = bool(np.intersect1d(ours, theirs, assume_unique=True).size)
+            got = b"overlap" in lib.t2_last_error()
+            assert got == want and (got or b"workspace" in lib.t2_last_error()), (B, T, H, sb, st, kw, lib.t2_last_error())
+            seen[want] += 1
+    assert min(seen) > 100, seen
