@@ -94,6 +94,9 @@ int t2_ctx_create(int device, void* hip_stream, t2_ctx** out);
 /* A context that enqueues on hip_stream itself, whatever it is: NULL is the device's default stream.  For callers whose other
  * work runs on that stream already: nothing has to be ordered against it.  The library never destroys the stream. */
 int t2_ctx_create_on_stream(int device, void* hip_stream, t2_ctx** out);
+/* "scan_wait_us" (default 2000000): how long a tile of t2_gated_scan / _backward waits for the tiles before it; behind that it computes
+ * what they would have handed over again from their inputs, bit for bit the same (0: at once, never waiting).  Of the calls to come. */
+int t2_ctx_set_option(t2_ctx* ctx, const char* name, int value);
 int t2_ctx_destroy(t2_ctx* ctx);
 int t2_ctx_synchronize(t2_ctx* ctx);
 
@@ -448,7 +451,8 @@ int t2_griffin_lim(t2_ctx* ctx, const float* spectrogram, int B, int T, int num_
  *     the state may overlap another tensor.
  * An output (y, the gradients, final_state, dstate, the tape that is written, ws) that overlaps itself, an input (z, f, o, dy, lens, state, dfinal, the
  * tape that is read, active) or another output is refused, whatever the strides.
- * All three only enqueue; none allocates, so they can be captured. */
+ * All three only enqueue; none allocates, so they can be captured.  Results do not depend on timing: tiles of a sequence wait for one
+ * another for a bounded time (t2_ctx_set_option), and one whose wait ends computes the missing state itself. */
 #define T2_F32 0
 #define T2_BF16 1
 #define T2_F16 2

@@ -76,6 +76,7 @@ _SIGS = {
     "t2_last_error": (C.c_char_p, []),
     "t2_ctx_create": (C.c_int, [C.c_int, _p, C.POINTER(_p)]),
     "t2_ctx_create_on_stream": (C.c_int, [C.c_int, _p, C.POINTER(_p)]),
+    "t2_ctx_set_option": (C.c_int, [_p, C.c_char_p, C.c_int]),
     "t2_ctx_destroy": (C.c_int, [_p]),
     "t2_ctx_synchronize": (C.c_int, [_p]),
     "t2_model_create": (C.c_int, [_p, C.POINTER(T2Dims), C.POINTER(_p)]),

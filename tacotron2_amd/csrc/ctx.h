@@ -28,6 +28,7 @@ struct t2_ctx {
     float* red_ws = nullptr;   // partial sums of the loss reductions (train.h)
     void* voc_ws = nullptr;    // Griffin-Lim workspace (vocoder.h), grown on demand
     size_t voc_ws_bytes = 0;
+    unsigned long long scan_wait_ticks = 200000000ull;     // option scan_wait_us, of the 100 MHz clock (recurrence.hip)
 };
 
 // Makes the context's device current for the length of a call and the caller's again behind it.

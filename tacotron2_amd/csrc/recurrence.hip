@@ -40,16 +40,18 @@ __device__ __forceinline__ int row_length(const int64_t* lens, int b, int T) {
 // carries its own validity (all ones: not there yet; a computed NaN is never that pattern), so one relaxed agent-scope access hands
 // it over, without flags or fences.  A workgroup's chain (row and channels) is
 // its index's, its tile is drawn from the chain's counter as it starts: it waits only for workgroups of the chain that have started
-// before it and that wait for none behind them, so every wait ends.  Every chain's counter has a line of its own: additions to one
-// address take 10 ns each.
+// before it and that wait for none behind them, so every wait ends.  A wave that was off the machine all the same (a GPU shared
+// between processes) waits no longer than the context's limit: it then composes the tiles before it once more from their inputs, with the
+// same operations in the same order, so the limit never changes a bit of a result (the last tile of T = 65536: 32 ms, backward 61).  Every chain's
+// counter has a line of its own: additions to one address take 10 ns each.
 // ------------------------------------------------------------------------------------------------
 #define SCAN_GROUP 8
-#define SCAN_WAIT_TICKS 200000000ull   /* 2 s of the 100 MHz clock; a wait never comes near it.  Beyond: NaN, not a hang */
 
 struct ScanWs {                        // counters [chains][16] | compositions [ntile][chains][CH] | states in front of the groups [ngroup][chains][CH]
     unsigned* next;
     unsigned long long* piece;
     unsigned* state;
+    unsigned long long ticks;          // of the 100 MHz clock that a wait may take; 0: nothing is waited for
 };
 static inline ScanWs scan_ws(void* p, long long chains, long long slots) {
     ScanWs w;
@@ -72,8 +74,9 @@ __device__ __forceinline__ void publish(unsigned* p, float v) { __hip_atomic_sto
 
 // The value that enters the i-th tile of a chain (i = 0: `first`), for one channel a lane.  slot: the tile's place among the
 // compositions (of the workgroup: the same for all lanes); hop: from one tile of the chain to the next; row: the group's place among
-// the states, row_hop: to the group before.
-__device__ __forceinline__ float look_back(const ScanWs& w, int i, float first, unsigned lane, long long slot, long long hop, long long row, long long row_hop) {
+// the states, row_hop: to the group before; again(): the same value without the other workgroups.
+template <typename Again>
+__device__ __forceinline__ float look_back(const ScanWs& w, int i, float first, unsigned lane, long long slot, long long hop, long long row, long long row_hop, Again again) {
     if (i == 0) return first;
     const bool head = i % SCAN_GROUP == 0;             // the first tile of a group folds the whole group before it
     const int m = head ? SCAN_GROUP : i % SCAN_GROUP, group = i / SCAN_GROUP - (head ? 1 : 0);
@@ -82,7 +85,8 @@ __device__ __forceinline__ float look_back(const ScanWs& w, int i, float first, 
     const unsigned long long t0 = __builtin_amdgcn_s_memrealtime();
     unsigned st = 0;
     unsigned long long pc[SCAN_GROUP];
-    for (;;) {
+    bool all = false, late = false;                    // late: one more look at everything, then no more
+    while (w.ticks > 0) {
         // all of it at once, each address a scalar base and the lane
         if (group > 0) st = __hip_atomic_load(start + lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 #pragma unroll
@@ -94,23 +98,28 @@ __device__ __forceinline__ float look_back(const ScanWs& w, int i, float first, 
         bool there = st != ~0u;
 #pragma unroll
         for (int k = 0; k < SCAN_GROUP; ++k) there = there && pc[k] != ~0ull;
-        if (__all(there)) break;
+        all = __all(there);
+        if (all || late) break;
         // not yet: wait for the tile before, then for the state, one word a lane at a time (waves that wait would otherwise read as
         // much as waves that work)
         const unsigned long long* before = w.piece + (slot - hop);
         bool wait = true;
-        while (wait) {
+        while (wait && !late) {
             __builtin_amdgcn_s_sleep(1);
             const unsigned long long v = __hip_atomic_load(before + lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             wait = !__all(v != ~0ull);
             if (!wait && group > 0) wait = !__all(__hip_atomic_load(start + lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != ~0u);
-            if (__builtin_amdgcn_s_memrealtime() - t0 > SCAN_WAIT_TICKS) return __builtin_nanf("");
+            late = __builtin_amdgcn_s_memrealtime() - t0 > w.ticks;
         }
     }
     float h = group > 0 ? __builtin_bit_cast(float, st) : first;
+    if (all) {
 #pragma unroll
-    for (int k = 0; k < SCAN_GROUP; ++k)
-        if (k < m) h = fmaf(__builtin_bit_cast(float, (unsigned)pc[k]), h, __builtin_bit_cast(float, (unsigned)(pc[k] >> 32)));
+        for (int k = 0; k < SCAN_GROUP; ++k)
+            if (k < m) h = fmaf(__builtin_bit_cast(float, (unsigned)pc[k]), h, __builtin_bit_cast(float, (unsigned)(pc[k] >> 32)));
+    } else {
+        h = again();
+    }
     if (head) publish(w.state + row + lane, h);
     return h;
 }
@@ -245,6 +254,43 @@ __device__ __forceinline__ void steps_of(const Inputs<E, L>& in, int i0, int row
     for (int j = 0; j < 4; ++j) piece[j] = make_float2(A[j], B[j]);
 }
 
+// The kernel's arguments out of their memory, for code that hardly ever runs: nothing of it is held in scalar registers before.
+typedef const __attribute__((address_space(4))) t2_scan_args* ArgsAgain;
+__device__ __forceinline__ ArgsAgain args_again() {
+    ArgsAgain a = (ArgsAgain)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(a));
+    return a;
+}
+
+// The state in front of the tile `tile` of channel cc: the pieces and compositions of the tiles before it, as those tiles make them.
+template <typename E, int TG, int L>
+__device__ __forceinline__ float states_again(int b, int len, int cc, int tile, float h) {
+    if (cc < 0) return h;
+    const ArgsAgain a = args_again();
+    const long long zs = a->reverse ? -a->z.stride_t : a->z.stride_t, fs = a->reverse ? -a->f.stride_t : a->f.stride_t;
+    long long z = b * a->z.stride_b + cc + (a->reverse ? len - 1 : 0) * a->z.stride_t, f = b * a->f.stride_b + cc + (a->reverse ? len - 1 : 0) * a->f.stride_t;
+#pragma unroll 1
+    for (int t = 0; t < tile; ++t) {
+        float At = 1.f, Bt = 0.f;
+#pragma unroll 1
+        for (int k = 0; k < TG; ++k) {
+            float A = 1.f, B = 0.f;
+#pragma unroll 1
+            for (int l = 0; l < L; ++l, z += zs, f += fs) {
+                float g, x;
+                gate(E::get(a->f.ptr, f), g, x);
+                x = x * E::get(a->z.ptr, z);
+                B = fmaf(g, B, x);
+                A *= g;
+            }
+            Bt = fmaf(A, Bt, B);
+            At *= A;
+        }
+        h = fmaf(At, h, Bt);
+    }
+    return h;
+}
+
 template <typename E, bool GATE, bool BUF, bool NT, int LANES, int L, int C>
 __device__ __forceinline__ void finish(const t2_scan_args& a, const Place<BUF, LANES, L>& t, int first, int rows, const Steps<L>& s, const typename E::Raw* o, f32v4 hin) {
     float h[4] = {hin[0], hin[1], hin[2], hin[3]};
@@ -297,7 +343,9 @@ __global__ __launch_bounds__(LANES* TG, WAVES) void scan_tile_kernel(t2_scan_arg
         const long long line = (long long)chains * CH, place = (long long)chain * CH, slot = tile * line + place;
         const bool more = first + C < t.len;                     // a tile behind this one will look back
         if (more) publish(w.piece + slot + lane, At, Bt);
-        const float h = look_back(w, tile, a.state && cc >= 0 ? a.state[(long long)t.b * a.H + cc] : 0.f, lane, slot, line, tile / SCAN_GROUP * line + place, line);
+        const float h0 = a.state && cc >= 0 ? a.state[(long long)t.b * a.H + cc] : 0.f;
+        const float h = look_back(w, tile, h0, lane, slot, line, tile / SCAN_GROUP * line + place, line,
+                                  [&] { return states_again<E, TG, L>(t.b, t.len, cc, tile, h0); });
         if (!more && a.final_state && cc >= 0) a.final_state[(long long)t.b * a.H + cc] = fmaf(At, h, Bt);
         distribute<TG, CH, false>(s_piece, s_in, lane, h);
     }
@@ -341,6 +389,41 @@ __device__ __forceinline__ void back_steps_of(const Grads<E, L>& in, int i0, int
         }
 #pragma unroll
     for (int j = 0; j < 4; ++j) { fwd[j] = make_float2(A[j], B[j]); bwd[j] = make_float2(A[j], Q[j]); }
+}
+
+// The gradient that enters the tile `tile` of channel cc from behind, out of the tiles behind it (the last of them may end early).
+template <typename E, bool GATE, int TG, int L>
+__device__ __forceinline__ float gradients_again(int b, int len, int cc, int last, int tile, float v) {
+    if (cc < 0) return v;
+    const ArgsAgain a = args_again();
+    const bool reverse = a->reverse;
+    auto place = [&](auto& q, int s) { return b * q.stride_b + (reverse ? len - 1 - s : s) * q.stride_t + cc; };
+#pragma unroll 1
+    for (int t = last; t > tile; --t) {
+        float At = 1.f, Qt = 0.f;
+#pragma unroll 1
+        for (int k = TG - 1; k >= 0; --k) {
+            const int first = (t * TG + k) * L, rows = len - first < L ? len - first : L;
+            float A = 1.f, Q = 0.f;
+#pragma unroll 1
+            for (int l = 0; l < rows; ++l) {
+                float g, x;
+                gate(E::get(a->f.ptr, place(a->f, first + l)), g, x);
+                A *= g;
+            }
+#pragma unroll 1
+            for (int l = rows - 1; l >= 0; --l) {
+                float g, x;
+                gate(E::get(a->f.ptr, place(a->f, first + l)), g, x);
+                const float dy = E::get(a->dy.ptr, place(a->dy, first + l));
+                Q = g * (GATE ? fmaf(dy, sigmoid1(E::get(a->o.ptr, place(a->o, first + l))), Q) : Q + dy);
+            }
+            Qt = fmaf(A, Qt, Q);
+            At *= A;
+        }
+        v = fmaf(At, v, Qt);
+    }
+    return v;
 }
 
 // the states in front of the pieces, from the tape's
@@ -445,7 +528,9 @@ __global__ __launch_bounds__(LANES* TG, WAVES) void scan_tile_backward_kernel(t2
         const int last = t.len > 0 ? (t.len - 1) / C : 0, at = last - tile;     // the last tile that is not all padding comes first
         const long long line = (long long)chains * CH, place = (long long)chain * CH, slot = tile * line + place;
         if (tile > 0) publish(w.piece + slot + lane, At, Qt);
-        const float l = look_back(w, at, a.dfinal && cc >= 0 ? a.dfinal[(long long)t.b * a.H + cc] : 0.f, lane, slot, -line, at / SCAN_GROUP * line + place, line);
+        const float l0 = a.dfinal && cc >= 0 ? a.dfinal[(long long)t.b * a.H + cc] : 0.f;
+        const float l = look_back(w, at, l0, lane, slot, -line, at / SCAN_GROUP * line + place, line,
+                                  [&] { return gradients_again<E, GATE, TG, L>(t.b, t.len, cc, last, tile, l0); });
         if (tile == 0 && a.dstate && cc >= 0) a.dstate[(long long)t.b * a.H + cc] = fmaf(At, l, Qt);
         distribute<TG, CH, true>(s_bwd, s_l, lane, l);
     }
@@ -650,6 +735,7 @@ static int launch(t2_ctx* ctx, const t2_scan_args* a) {
     ScanWs w = {};
     if (ntile > 1) {
         w = scan_ws(a->ws, blocks / ntile, blocks * CH);
+        w.ticks = ctx->scan_wait_ticks;
         const long long n16 = ws_bytes(a->B, a->T, a->H, tile) / 16, nb = (n16 + 1023) / 1024;
         hipLaunchKernelGGL(scan_ws_kernel, dim3((unsigned)(nb < 2048 ? nb : 2048)), dim3(256), 0, ctx->stream, (uint4*)a->ws, blocks / ntile * 4, n16);
     }

@@ -388,6 +388,14 @@ extern "C" int t2_ctx_create_on_stream(int device, void* hip_stream, t2_ctx** ou
     return ctx_create(device, (hipStream_t)hip_stream, false, out);
 }
 
+extern "C" int t2_ctx_set_option(t2_ctx* c, const char* name, int value) {
+    if (!c || !name) return fail(T2_EINVAL, "null argument");
+    if (strcmp(name, "scan_wait_us")) return fail(T2_EINVAL, "unknown option '%s'", name);
+    if (value < 0) return fail(T2_EINVAL, "scan_wait_us is %d", value);
+    c->scan_wait_ticks = (unsigned long long)value * 100;
+    return T2_OK;
+}
+
 extern "C" int t2_ctx_destroy(t2_ctx* c) {
     if (!c) return T2_OK;
     if (c->red_ws) (void)hipFree(c->red_ws);

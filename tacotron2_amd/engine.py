@@ -101,6 +101,10 @@ class Context:
         self.handle = C.c_void_p()
         _lib.check(self.lib.t2_ctx_create(device, C.c_void_p(self.stream.cuda_stream), C.byref(self.handle)))
 
+    def set_option(self, name: str, value: int):
+        """``scan_wait_us``: include/t2mi.h, t2_ctx_set_option."""
+        _lib.check(self.lib.t2_ctx_set_option(self.handle, name.encode(), int(value)))
+
     def f32(self, x) -> torch.Tensor:
         if not isinstance(x, torch.Tensor):
             x = torch.as_tensor(np.asarray(x, dtype=np.float32))

@@ -24,3 +24,29 @@ def test_a_state_that_lies_in_the_output(T):
     lens = out.view(torch.int64).view(-1)[:1]
     with pytest.raises(T2Error):
         R.gated_scan(None, z, f, lens=lens, out=out)
+
+
+@pytest.mark.parametrize("dtype,B,T,H,gate,reverse", [("f32", 2, 700, 36, True, False), ("bf16", 3, 1500, 130, True, True), ("f16", 1, 2300, 3, False, True),
+                                                      ("f32", 1, 5000, 66, False, False), ("bf16", 8, 12300, 512, True, True)])
+def test_a_tile_that_does_not_wait_gets_the_same_bits(dtype, B, T, H, gate, reverse):
+    """scan_wait_us 0: every tile computes what enters it from the inputs of the tiles before it; 1: some do."""
+    from tacotron2_amd import recurrence as R
+    from tacotron2_amd.engine import Context
+    gen = torch.Generator(device="cuda").manual_seed(T)
+    r = lambda *s: torch.randn(s, generator=gen, device="cuda")  # noqa: E731
+    dt = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}[dtype]
+    z, f, dy = r(B, T, H).to(dt), (r(B, T, H) * 1.5 + 4).to(dt), r(B, T, H).to(dt)
+    o = r(B, T, H).to(dt) if gate else None
+    state, dfinal = r(B, H), r(B, H)
+    ctx = Context(0)
+    for lens in (None, torch.tensor([T - 301 * b for b in range(B)], device="cuda").clamp(min=0)):
+        got = []
+        for us in (2_000_000, 0, 1):
+            ctx.set_option("scan_wait_us", us)
+            y, final, tape = R.gated_scan(ctx, z, f, o, lens=lens, state=state, reverse=reverse, tape=True)
+            dz, df, do, dstate = R.gated_scan_backward(ctx, tape, dy, dfinal)
+            got.append([y, final, tape.states if lens is None else final, dz, df, dz if do is None else do, dstate])
+        for other in got[1:]:
+            for a, b in zip(got[0], other):
+                assert torch.isfinite(a).all() and torch.equal(a, b)
+    ctx.close()

@@ -170,3 +170,11 @@ def test_overlaps_of_different_strides_are_found_exactly():
             assert got == want and (got or b"workspace" in lib.t2_last_error()), (B, T, H, sb, st, kw, lib.t2_last_error())
             seen[want] += 1
     assert min(seen) > 100, seen
+
+
+def test_context_options():
+    lib = _lib.load()
+    ctx = C.create_string_buffer(256)                # takes the option's value; no device work
+    assert lib.t2_ctx_set_option(ctx, b"scan_wait_us", 0) == _lib.T2_OK and lib.t2_ctx_set_option(ctx, b"scan_wait_us", 2000000) == _lib.T2_OK
+    for bad in ((None, b"scan_wait_us", 1), (ctx, None, 1), (ctx, b"scan_wait", 1), (ctx, b"scan_wait_us", -1)):
+        assert lib.t2_ctx_set_option(*bad) == _lib.T2_EINVAL, bad
