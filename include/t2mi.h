@@ -480,7 +480,7 @@ int t2_gated_scan_step(t2_ctx* ctx, int dtype, int B, int H, const void* z, int6
 
 /* ---- AdamW over many tensors at once (beside t2_optim_*; the reference's optimizer is TF's Adam without decay) ---------------------
  * One step of decoupled weight decay over n_tensors tensors of fp32, bf16 or fp16 (parameters and gradients each in a type of their own):
- *     g' = gs g, gs = grad_scale * clip / max(grad_scale * |g|, clip) with the norm over all tensors (clip <= 0: gs = grad_scale)
+ *     g' = gs g, gs = grad_scale * clip / max(grad_scale * |g|, clip) with the norm over all tensors (clip <= 0 or inf: gs = grad_scale)
  *     m' = b1 m + (1 - b1) g'      v' = b2 v + (1 - b2) g'^2
  *     p' = p (1 - lr decay) - lr / (1 - b1^t) * m' / (sqrt(v' / (1 - b2^t)) + epsilon)
  * Arithmetic is fp32 (the norm and the factors of a step: double); p' is rounded once to the parameter's type and once to its copy's.
@@ -492,6 +492,7 @@ int t2_gated_scan_step(t2_ctx* ctx, int dtype, int B, int H, const void* z, int6
  *  - t2_adamw_bind writes a table (dev, t2_adamw_table_bytes(), 16-byte aligned) of the tensors' addresses and types on the stream; the
  *    other calls for the same handle read it (a table of another handle has another number of tensors: never give it).  params may be
  *    NULL for a table that only serves the norm; copies (NULL, or NULL entries) get p' in their own type.
+ *  - grad_scale and learning_rate have to be fp32 numbers (no inf, no NaN), clip_norm no NaN.
  *  - learning_rate_dev: dev float that replaces learning_rate, or NULL.  skip_nonfinite: a step whose gradient norm is inf or NaN changes
  *    nothing and is not counted.  Without it a NaN reaches the elements that have it (and their blocks of 128 in 8 bits).
  * Calls for one handle must follow one another on the device; the handle's workspace belongs to the call that runs. */

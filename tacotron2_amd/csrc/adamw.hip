@@ -9,6 +9,8 @@
 #include "elem.h"
 #include "rng.h"
 
+#include <float.h>
+#include <math.h>
 #include <new>
 #include <vector>
 
@@ -114,7 +116,7 @@ __device__ void begin_step(const AwNormArgs& a, double norm) {
     *a.step = t;
     const double lr = a.lr_dev ? (double)*a.lr_dev : a.lr;
     c.t = (uint32_t)t;
-    c.gs = (float)(a.clip > 0.0 ? a.grad_scale * (a.clip / fmax(norm, a.clip)) : a.grad_scale);
+    c.gs = (float)(a.clip > 0.0 && norm > a.clip ? a.grad_scale * (a.clip / norm) : a.grad_scale);     // a limit of inf: no limit
     c.lr = (float)lr;
     c.lr_t = (float)(lr / (1.0 - power(a.b1, t)));
     c.ic2 = (float)(1.0 / sqrt(1.0 - power(a.b2, t)));
@@ -483,7 +485,11 @@ static void launch_norm(const t2_ctx* ctx, const t2_adamw* o, const AwNormArgs& 
     else hipLaunchKernelGGL(adamw_norm_kernel<false>, grid, threads, 0, ctx->stream, a);
 }
 
+// the factors of a step are fp32 on the device
+static bool fits_f32(double x) { return fabs(x) <= FLT_MAX; }
+
 extern "C" int t2_adamw_global_norm(t2_ctx* ctx, t2_adamw* o, const void* table, double grad_scale, float* norm_out) {
+    if (!fits_f32(grad_scale)) return fail(T2_EINVAL, "grad_scale is %g", grad_scale);
     T2_TRY(check_call(ctx, o));
     if (!table || !norm_out) return fail(T2_EINVAL, "null argument");
     DeviceScope dev(ctx->device);
@@ -497,6 +503,9 @@ extern "C" int t2_adamw_global_norm(t2_ctx* ctx, t2_adamw* o, const void* table,
 
 extern "C" int t2_adamw_step(t2_ctx* ctx, t2_adamw* o, const void* table, double learning_rate, const float* learning_rate_dev, double clip_norm,
                              double grad_scale, int skip_nonfinite) {
+    if (!fits_f32(grad_scale)) return fail(T2_EINVAL, "grad_scale is %g", grad_scale);
+    if (!learning_rate_dev && !fits_f32(learning_rate)) return fail(T2_EINVAL, "learning_rate is %g", learning_rate);
+    if (clip_norm != clip_norm) return fail(T2_EINVAL, "clip_norm is NaN");
     T2_TRY(check_call(ctx, o));
     if (!table) return fail(T2_EINVAL, "null argument");
     DeviceScope dev(ctx->device);

@@ -400,7 +400,7 @@ class AdamW:
     def apply_gradients(self, grads, params=None, global_step: int = 0, clip_norm: float = 1.0, grad_scale: float = 1.0, copies=None,
                         skip_nonfinite: bool = False) -> int:
         """One step on ``params`` in place (``grads``: tensors, or an AdamWBinding of gradients and parameters); returns global_step + 1.
-        ``clip_norm <= 0`` does not clip.  ``skip_nonfinite``: gradients whose norm is inf or NaN change nothing (``steps()`` stays)."""
+        ``clip_norm <= 0`` or inf does not clip.  ``skip_nonfinite``: gradients whose norm is inf or NaN change nothing (``steps()`` stays)."""
         if isinstance(grads, AdamWBinding):
             b = grads
             if params is not None or copies is not None:

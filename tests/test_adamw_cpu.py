@@ -85,3 +85,12 @@ def test_a_binding_serves_its_own_optimizer_only():
         few.apply_gradients(b)
     for o in (few, many, same):
         o._h = None                                          # nothing of the library's to give back
+
+
+def test_factors_that_are_no_numbers_are_refused():
+    lib = _lib.load()
+    nan, inf = float("nan"), float("inf")
+    for lr, clip, scale, what in ((nan, 1.0, 1.0, b"learning_rate"), (inf, 1.0, 1.0, b"learning_rate"), (1e39, 1.0, 1.0, b"learning_rate"), (1e-3, nan, 1.0, b"clip_norm"),
+                                  (1e-3, 1.0, nan, b"grad_scale"), (1e-3, 1.0, -inf, b"grad_scale"), (1e-3, 1.0, 1e39, b"grad_scale")):
+        assert lib.t2_adamw_step(None, None, None, lr, None, clip, scale, 0) == _lib.T2_EINVAL and what in lib.t2_last_error(), what
+    assert lib.t2_adamw_global_norm(None, None, None, nan, None) == _lib.T2_EINVAL and b"grad_scale" in lib.t2_last_error()
