@@ -492,6 +492,7 @@ int t2_gated_scan_step(t2_ctx* ctx, int dtype, int B, int H, const void* z, int6
  *  - t2_adamw_bind writes a table (dev, t2_adamw_table_bytes(), 16-byte aligned) of the tensors' addresses and types on the stream; the
  *    other calls for the same handle read it (a table of another handle has another number of tensors: never give it).  params may be
  *    NULL for a table that only serves the norm; copies (NULL, or NULL entries) get p' in their own type.
+ *  - epsilon is 1.2e-38 (the smallest normal fp32 number) or more.
  *  - grad_scale and learning_rate have to be fp32 numbers (no inf, no NaN), clip_norm no NaN.
  *  - learning_rate_dev: dev float that replaces learning_rate, or NULL.  skip_nonfinite: a step whose gradient norm is inf or NaN changes
  *    nothing and is not counted.  Without it a NaN reaches the elements that have it (and their blocks of 128 in 8 bits).

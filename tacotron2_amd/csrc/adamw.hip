@@ -409,7 +409,9 @@ extern "C" int t2_adamw_create(t2_ctx* ctx, int n_tensors, const int64_t* sizes,
                                int state_bits, uint32_t seed, void* m, void* v, void* m_scale, void* v_scale, int64_t* step, t2_adamw** out) {
     if (!ctx || !sizes || !decay || !m || !v || !step || !out) return fail(T2_EINVAL, "null argument");
     if (t2_adamw_elements(n_tensors, sizes) < 0) return T2_EINVAL;
-    if (!(beta1 >= 0.0 && beta1 < 1.0) || !(beta2 >= 0.0 && beta2 < 1.0) || !(epsilon > 0.0)) return fail(T2_EINVAL, "AdamW needs 0 <= beta < 1 and epsilon > 0");
+    // the reciprocal of epsilon is a number: an element whose moments are zero stays where it is
+    if (!(beta1 >= 0.0 && beta1 < 1.0) || !(beta2 >= 0.0 && beta2 < 1.0) || !((float)epsilon >= FLT_MIN && (float)epsilon <= FLT_MAX))
+        return fail(T2_EINVAL, "AdamW needs 0 <= beta < 1 and an epsilon from 1.2e-38 on");
     if (state_bits != 32 && state_bits != 8) return fail(T2_EINVAL, "states have 32 or 8 bits, not %d", state_bits);
     if (state_bits == 8 && (!m_scale || !v_scale)) return fail(T2_EINVAL, "states in 8 bits need scales");
     if ((((uintptr_t)m) | ((uintptr_t)v)) & 15) return fail(T2_EINVAL, "the states must be 16-byte aligned");

@@ -295,7 +295,7 @@ class AdamW:
     the next forward pass reads) get the new values in their type in the same pass.  ``state_bits=32``: fp32 moments.  ``state_bits=8``:
     ``m`` and the root of ``v`` as float8_e4m3fn with one power of two (float8_e8m0fnu) for 128 elements, rounded stochastically by
     (``seed``, step, element): 2 bytes an element in place of 8.  The difference from AdamOptimizer's TF form: bias corrections on both
-    moments, epsilon beside the corrected root, weight decay.
+    moments, epsilon (1.2e-38 or more) beside the corrected root, weight decay.
 
     ``m``, ``v``, ``m_scale``, ``v_scale`` are the live states, tensor i's from ``offsets[i]`` on (``load_state`` sets them).  The step count is
     on the device (``steps()``), so a captured step counts at every replay; capture with a learning rate that is a device scalar

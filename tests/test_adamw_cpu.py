@@ -94,3 +94,12 @@ def test_factors_that_are_no_numbers_are_refused():
                                   (1e-3, 1.0, nan, b"grad_scale"), (1e-3, 1.0, -inf, b"grad_scale"), (1e-3, 1.0, 1e39, b"grad_scale")):
         assert lib.t2_adamw_step(None, None, None, lr, None, clip, scale, 0) == _lib.T2_EINVAL and what in lib.t2_last_error(), what
     assert lib.t2_adamw_global_norm(None, None, None, nan, None) == _lib.T2_EINVAL and b"grad_scale" in lib.t2_last_error()
+
+
+def test_an_epsilon_that_fp32_cannot_invert_is_refused():
+    lib = _lib.load()
+    ctx, out, buf = C.create_string_buffer(64), C.c_void_p(), C.create_string_buffer(64)
+    at = (C.addressof(buf) + 15) & ~15
+    for eps in (1e-46, 1e-39, 1.17e-38, 1e39, float("inf"), float("nan"), -1e-8):
+        assert lib.t2_adamw_create(ctx, 1, (C.c_int64 * 1)(5), (C.c_double * 1)(0.0), 0.9, 0.999, eps, 32, 0, at, at, None, None, at, C.byref(out)) == _lib.T2_EINVAL, eps
+        assert b"epsilon" in lib.t2_last_error()

@@ -1,4 +1,5 @@
 """AdamW with the smallest and largest factors, scales and tables that its documentation allows."""
+import numpy as np
 import pytest
 
 pytestmark = pytest.mark.gpu
@@ -38,3 +39,17 @@ def test_an_infinite_limit_does_not_clip(bits):
         assert torch.equal(x, y)
     for o in (a, b):
         o.close()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_elements_without_a_gradient_stay_with_the_smallest_epsilon(bits):
+    eps = float(np.finfo(np.float32).tiny)
+    opt, _ = _make([300], bits, decay=[0.0], epsilon=eps)
+    p = _tensors([300], ["f32"], 1)
+    g = torch.zeros(300, device="cuda")
+    g[:128] = torch.randn(128, generator=torch.Generator().manual_seed(2)).cuda()
+    before = p[0].clone()
+    for _ in range(2):
+        opt.apply_gradients([g], p, clip_norm=0.0)
+    assert torch.isfinite(p[0]).all() and torch.equal(p[0][128:], before[128:]) and not torch.equal(p[0][:128], before[:128])
+    opt.close()
