@@ -230,6 +230,21 @@ __device__ __forceinline__ void decode8(u32v2 codes, int scale, float* x) {
     }
 }
 
+// Roots within an ulp.  The instruction takes subnormal numbers for zeros (gradients under 1e-17 with an epsilon that small too would be
+// divided by epsilon alone): they go through it larger by 2^32.
+__device__ __forceinline__ void roots_within_an_ulp(const float* x, float* r) {
+    float least = x[0];
+#pragma unroll
+    for (int j = 1; j < AW_VEC; ++j) least = fminf(least, x[j]);
+    if (__all(least >= 0x1p-96f)) {
+#pragma unroll
+        for (int j = 0; j < AW_VEC; ++j) r[j] = __builtin_amdgcn_sqrtf(x[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < AW_VEC; ++j) r[j] = x[j] < 0x1p-96f ? __builtin_amdgcn_sqrtf(x[j] * 0x1p32f) * 0x1p-16f : __builtin_amdgcn_sqrtf(x[j]);
+    }
+}
+
 // The correctly rounded root of every element.  With x normal: from the reciprocal root (one ulp) one correction by the exact residual,
 // a third of what the general function takes; zeros and numbers too small or large for it go
 // through that.
@@ -328,8 +343,7 @@ __global__ __launch_bounds__(AW_THREADS) void adamw_step_kernel(AwStepArgs a) {
         if constexpr (BITS == 8) {
             roots(v, r);
         } else {
-#pragma unroll
-            for (int j = 0; j < AW_VEC; ++j) r[j] = __builtin_amdgcn_sqrtf(v[j]);
+            roots_within_an_ulp(v, r);
         }
 #pragma unroll
         for (int j = 0; j < AW_VEC; ++j) p[j] = p[j] * keep - lr_t * m[j] * __builtin_amdgcn_rcpf(r[j] * ic2 + a.eps);

@@ -53,3 +53,23 @@ def test_elements_without_a_gradient_stay_with_the_smallest_epsilon(bits):
         opt.apply_gradients([g], p, clip_norm=0.0)
     assert torch.isfinite(p[0]).all() and torch.equal(p[0][128:], before[128:]) and not torch.equal(p[0][:128], before[:128])
     opt.close()
+
+
+def test_roots_of_subnormal_second_moments():
+    """Gradients of 1e-21 to 1e-17: v is subnormal or next to it, and with an epsilon of 1e-30 the root of v alone is the divisor.  The
+    state is the formula's in fp32, bit for bit; from there the update passes lr_t, m, two products, a root and a reciprocal of one ulp
+    each, a product and a sum: less than 12 roundings."""
+    n = 4096
+    lr, b1, b2, eps = 1e-2, 0.9, 0.99, 1e-30
+    opt, _ = _make([n], 32, decay=[0.0], epsilon=eps)
+    rng = np.random.default_rng(4)
+    x = (rng.choice([-1.0, 1.0], n) * 10.0 ** rng.uniform(-21, -17, n)).astype(np.float32)
+    g, p = torch.from_numpy(x).cuda(), torch.zeros(n, device="cuda")
+    opt.apply_gradients([g], [p], clip_norm=0.0)
+    with np.errstate(under="ignore"):
+        v = (x * x) * np.float32(1 - b2)
+    assert np.array_equal(opt.v[:n].cpu().numpy(), v)
+    want = -(lr / (1 - b1)) * ((1 - b1) * x.astype(np.float64)) / (np.sqrt(v.astype(np.float64)) / np.sqrt(1 - b2) + eps)
+    off = np.abs(p.double().cpu().numpy() - want)
+    assert (off <= 12 * 2.0 ** -24 * np.abs(want)).all(), float((off / np.abs(want)).max())
+    opt.close()
