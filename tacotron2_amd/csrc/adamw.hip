@@ -222,7 +222,7 @@ __device__ __forceinline__ uint32_t row_max(uint32_t x) {      // over the 16 la
 // Eight values: two at a time by the converter, times the block's power of two (255: NaN, which the product keeps).  Both are exact.
 __device__ __forceinline__ void decode8(u32v2 codes, int scale, float* x) {
     typedef float F2 __attribute__((ext_vector_type(2)));
-    const float power = scale == 255 ? __builtin_nanf("") : __builtin_bit_cast(float, (uint32_t)scale << 23);
+    const float power = scale == 255 ? __builtin_nanf("") : __builtin_bit_cast(float, scale ? (uint32_t)scale << 23 : 0x400000u);      // 0: 2^-127, subnormal
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const F2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes[h], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes[h], true);

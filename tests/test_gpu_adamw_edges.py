@@ -4,6 +4,7 @@ import pytest
 
 pytestmark = pytest.mark.gpu
 
+from tests import adamw_ref as ref
 from tests.test_gpu_adamw import _make, _tensors
 
 torch = pytest.importorskip("torch")
@@ -72,4 +73,22 @@ def test_roots_of_subnormal_second_moments():
     want = -(lr / (1 - b1)) * ((1 - b1) * x.astype(np.float64)) / (np.sqrt(v.astype(np.float64)) / np.sqrt(1 - b2) + eps)
     off = np.abs(p.double().cpu().numpy() - want)
     assert (off <= 12 * 2.0 ** -24 * np.abs(want)).all(), float((off / np.abs(want)).max())
+    opt.close()
+
+
+def test_the_smallest_scale_of_loaded_states():
+    """A scale byte of 0 is 2^-127, as every other one is 2^(byte - 127)."""
+    opt, _ = _make([512], 8, decay=[0.0], seed=11)
+    rng = np.random.default_rng(7)
+    codes = rng.integers(0, 0x7F, 512).astype(np.uint8) | (rng.integers(0, 2, 512).astype(np.uint8) << 7)
+    roots = rng.integers(0, 0x7F, 512).astype(np.uint8)
+    ms, vs = np.array([0, 1, 0, 20], np.uint8), np.array([0, 0, 90, 1], np.uint8)
+    dev = lambda a, dt: torch.from_numpy(a).cuda().view(dt)  # noqa: E731
+    opt.load_state(dev(codes, torch.float8_e4m3fn), dev(roots, torch.float8_e4m3fn), 4, m_scale=dev(ms, torch.float8_e8m0fnu), v_scale=dev(vs, torch.float8_e8m0fnu))
+    p, g = torch.zeros(512, device="cuda"), torch.zeros(512, device="cuda")
+    opt.apply_gradients([g], [p], clip_norm=0.0)
+    raw = lambda t: t.view(torch.uint8).cpu().numpy()  # noqa: E731
+    mc, msn, vc, vsn, _, _ = ref.step8(codes, ms, roots, vs, np.zeros(512, np.float32), 5, 1.0, 0.9, 0.99, opt.seed, 0)
+    assert mc[:128].any() and np.array_equal(raw(opt.m), mc) and np.array_equal(raw(opt.m_scale), msn)
+    assert np.array_equal(raw(opt.v), vc) and np.array_equal(raw(opt.v_scale), vsn)
     opt.close()
