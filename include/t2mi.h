@@ -444,6 +444,8 @@ int t2_griffin_lim(t2_ctx* ctx, const float* spectrogram, int B, int T, int num_
  *  - ws: dev buffer of t2_gated_scan_ws() bytes, 16-byte aligned, used by this call only (no content is kept between calls: two captured
  *    graphs that may run at once need a buffer each).
  * Gates, state and sums are fp32 whatever the type; y and the gradients are rounded once.
+ * An infinite z, state or gradient keeps h (or its gradient) infinite from there on; NaN spreads along its own row and channel, in the
+ * direction of the recurrence.
  * t2_gated_scan_backward: dy [B][T][H] of the same type, dfinal dev fp32 [B][H] or NULL (the gradient of final_state) ->
  *     dz, df, do (do where o was given), dstate (dev fp32 [B][H] or NULL); zeros at positions behind a row's length.
  * t2_gated_scan_step: one new position for each row, z, f, o, y [B][H] (stride_b only), state dev fp32 [B][H] with a row stride, updated in place.

@@ -197,6 +197,10 @@ __device__ __forceinline__ unsigned chain_of(unsigned index, unsigned chains) {
     return chains % 8 == 0 ? c % 8 * (chains / 8) + c / 8 : c;
 }
 
+// A product of gates in fp32 reaches zero where the gates do not, and zero times an infinite h would be NaN: the smallest number instead
+// keeps h infinite, as every single step does, and is nothing beside any other h.
+__device__ __forceinline__ float product(float A) { return fmaxf(A, 0x1p-149f); }
+
 // the composition of all TG pieces of a channel, in the order of the steps or against it
 template <int TG, int CH, bool BACK>
 __device__ __forceinline__ void compose(const float2 (*piece)[CH], unsigned lane, float& A, float& B) {
@@ -207,6 +211,7 @@ __device__ __forceinline__ void compose(const float2 (*piece)[CH], unsigned lane
         B = fmaf(p.x, B, p.y);
         A *= p.x;
     }
+    A = product(A);
     asm volatile("" ::: "memory");                         // distribute() reads the pieces again: 2 TG registers otherwise
 }
 // v, which enters the tile, taken through the pieces: what enters each of them goes to `in`; returns what leaves
@@ -251,7 +256,7 @@ __device__ __forceinline__ void steps_of(const Inputs<E, L>& in, int i0, int row
             A[j] *= s.a[l][j];
         }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) piece[j] = make_float2(A[j], B[j]);
+    for (int j = 0; j < 4; ++j) piece[j] = make_float2(product(A[j]), B[j]);
 }
 
 // The kernel's arguments out of their memory, for code that hardly ever runs: nothing of it is held in scalar registers before.
@@ -283,10 +288,11 @@ __device__ __forceinline__ float states_again(int b, int len, int cc, int tile, 
                 B = fmaf(g, B, x);
                 A *= g;
             }
+            A = product(A);
             Bt = fmaf(A, Bt, B);
             At *= A;
         }
-        h = fmaf(At, h, Bt);
+        h = fmaf(product(At), h, Bt);
     }
     return h;
 }
@@ -388,7 +394,7 @@ __device__ __forceinline__ void back_steps_of(const Grads<E, L>& in, int i0, int
             Q[j] = s.a[l][j] * (GATE ? fmaf(dy, sigmoid1(E::at(in.o[l], j)), Q[j]) : Q[j] + dy);
         }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) { fwd[j] = make_float2(A[j], B[j]); bwd[j] = make_float2(A[j], Q[j]); }
+    for (int j = 0; j < 4; ++j) { fwd[j] = make_float2(product(A[j]), B[j]); bwd[j] = make_float2(fwd[j].x, Q[j]); }
 }
 
 // The gradient that enters the tile `tile` of channel cc from behind, out of the tiles behind it (the last of them may end early).
@@ -418,10 +424,11 @@ __device__ __forceinline__ float gradients_again(int b, int len, int cc, int las
                 const float dy = E::get(a->dy.ptr, place(a->dy, first + l));
                 Q = g * (GATE ? fmaf(dy, sigmoid1(E::get(a->o.ptr, place(a->o, first + l))), Q) : Q + dy);
             }
+            A = product(A);
             Qt = fmaf(A, Qt, Q);
             At *= A;
         }
-        v = fmaf(At, v, Qt);
+        v = fmaf(product(At), v, Qt);
     }
     return v;
 }

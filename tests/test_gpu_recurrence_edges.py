@@ -50,3 +50,46 @@ def test_a_tile_that_does_not_wait_gets_the_same_bits(dtype, B, T, H, gate, reve
             for a, b in zip(got[0], other):
                 assert torch.isfinite(a).all() and torch.equal(a, b)
     ctx.close()
+
+
+@pytest.mark.parametrize("dtype,B,T,H", [("f32", 2, 60, 12), ("bf16", 2, 200, 12), ("f32", 2, 1500, 12), ("f16", 3, 700, 3), ("f32", 9, 250, 2048)])
+@pytest.mark.parametrize("reverse", [False, True])
+def test_an_infinity_stays_one(dtype, B, T, H, reverse):
+    """Behind an infinite value or state h is infinite for good, however small the product of the gates since then has become; the
+    gradients likewise behind an infinite gradient.  Channels without one are what they were."""
+    z, f, o, state, dy, dfinal = _inputs(B, T, H, dtype, True, T)
+    f[..., 0] = -20.0                                                     # a product of four of these gates is below 2^-115
+    plain = _check(z, f, o, None, state, dy, dfinal, reverse, dtype)
+    inf = float("inf")
+    z[0, T // 3, 0], z[1, T // 2, 1], state[0, 1], state[1, 2] = inf, -inf, inf, -inf
+    _, final, _ = _check(z, f, o, None, state, dy, dfinal, reverse, dtype)
+    assert final[0, 0] == inf and final[1, 1] == -inf and final[0, 1] == inf and final[1, 2] == -inf
+    from tacotron2_amd.engine import Context
+    ctx = Context(0)
+    ctx.set_option("scan_wait_us", 0)
+    _check(z, f, o, None, state, dy, dfinal, reverse, dtype, ctx=ctx)
+    z, f, o, state, dy, dfinal = _inputs(B, T, H, dtype, True, T)
+    f[..., 0] = -20.0
+    dy[0, T // 3, 0], dy[1, T // 2, 1], dfinal[0, 1], dfinal[1, 2] = inf, -inf, inf, -inf
+    y, final, (dz, df, do, dstate) = _check(z, f, o, None, state, dy, dfinal, reverse, dtype)
+    assert dstate[0, 0] == inf and dstate[1, 1] == -inf and dstate[0, 1] == inf and dstate[1, 2] == -inf
+    _check(z, f, o, None, state, dy, dfinal, reverse, dtype, ctx=ctx)
+    ctx.close()
+    assert torch.equal(y, plain[0]) and torch.equal(final, plain[1])
+    for got, want in zip((dz, df, do), plain[2]):
+        assert torch.equal(got[..., 3:], want[..., 3:])
+
+
+def test_an_infinity_stays_one_in_large_calls():
+    """The same across the wide tiles of a large call."""
+    from tacotron2_amd import recurrence as R
+    B, T, H = 8, 12300, 512
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    r = lambda *s: torch.randn(s, generator=gen, device="cuda")  # noqa: E731
+    z, f, dy, dfinal = r(B, T, H).bfloat16(), (r(B, T, H) - 1).bfloat16(), r(B, T, H).bfloat16(), r(B, H)
+    inf = float("inf")
+    z[1, 5000, 130], dfinal[2, 300] = inf, -inf
+    y, final, tape = R.gated_scan(None, z, f, tape=True)
+    dz, _, _, dstate = R.gated_scan_backward(None, tape, dy, dfinal)
+    assert (y[1, 5000:, 130] == inf).all() and final[1, 130] == inf and (dz[2, :, 300] == -inf).all() and dstate[2, 300] == -inf
+    assert int(torch.isfinite(y).logical_not().sum()) == T - 5000 and int(torch.isfinite(dz).logical_not().sum()) == T
