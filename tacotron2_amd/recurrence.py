@@ -23,13 +23,21 @@ _DTYPES = {torch.float32: _lib.T2_F32, torch.bfloat16: _lib.T2_BF16, torch.float
 
 class ScanTape(NamedTuple):
     """What ``gated_scan_backward`` needs of a forward call: its inputs (not copied: leave them as they are until then) and the
-    states in front of every 64th step."""
+    states in front of every 64th step.  A backward pass on another stream (which the caller orders behind the forward call) keeps
+    their memory from being given away before that stream is done with it, so the tape can be dropped at once."""
     z: torch.Tensor
     f: torch.Tensor
     o: Optional[torch.Tensor]
     lens: Optional[torch.Tensor]
     reverse: bool
     states: torch.Tensor
+    stream: Optional[int] = None          # the forward call's: torch's current stream then
+
+    def _used(self):
+        if self.stream is None or torch._C._cuda_getCurrentRawStream(self.states.get_device()) != self.stream:
+            for t in (self.z, self.f, self.o, self.lens, self.states):
+                if t is not None:
+                    t.record_stream(torch.cuda.current_stream(self.states.device))
 
 
 def _context(ctx, t: torch.Tensor) -> Context:
@@ -136,7 +144,7 @@ def gated_scan(ctx, z, f, o=None, lens=None, state=None, reverse: bool = False, 
                                final.data_ptr(), _ptr(states), *_NONE, *_NONE, *_NONE, *_NONE, 0, 0, _ptr(ws), n))
     with ctx.ordered():
         _lib.check(ctx.lib.t2_gated_scan(ctx.handle, args))
-    return (y, final, ScanTape(z, f, o, lens, bool(reverse), states)) if tape else (y, final)
+    return (y, final, ScanTape(z, f, o, lens, bool(reverse), states, torch._C._cuda_getCurrentRawStream(device.index))) if tape else (y, final)
 
 
 def gated_scan_backward(ctx, tape: ScanTape, dy, dfinal=None):
@@ -157,6 +165,7 @@ def gated_scan_backward(ctx, tape: ScanTape, dy, dfinal=None):
     ws, n = _workspace(ctx, B, T, H)
     args = _lib.T2ScanArgs.from_buffer_copy(_lib.SCAN_ARGS.pack(_DTYPES[z.dtype], B, T, H, int(tape.reverse), *_seq(z), *_seq(tape.f), *_seq(tape.o), *_NONE, _ptr(tape.lens), 0, 0,
                                tape.states.data_ptr(), *_seq(dy), *_seq(dz), *_seq(df), *_seq(do), _ptr(dfinal), dstate.data_ptr(), _ptr(ws), n))
+    tape._used()
     with ctx.ordered():
         _lib.check(ctx.lib.t2_gated_scan_backward(ctx.handle, args))
     return dz, df, do, dstate

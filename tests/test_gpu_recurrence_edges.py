@@ -93,3 +93,30 @@ def test_an_infinity_stays_one_in_large_calls():
     dz, _, _, dstate = R.gated_scan_backward(None, tape, dy, dfinal)
     assert (y[1, 5000:, 130] == inf).all() and final[1, 130] == inf and (dz[2, :, 300] == -inf).all() and dstate[2, 300] == -inf
     assert int(torch.isfinite(y).logical_not().sum()) == T - 5000 and int(torch.isfinite(dz).logical_not().sum()) == T
+
+
+@pytest.mark.parametrize("lens", [None, [2000, 3]])
+def test_a_tape_used_on_another_stream_and_dropped_at_once(lens):
+    from tacotron2_amd import recurrence as R
+    z, f, o, state, dy, dfinal = _inputs(2, 2000, 300, "f32", True, 6)
+    _, _, tape = R.gated_scan(None, z, f, o, lens=lens, state=state, tape=True)
+    want = R.gated_scan_backward(None, tape, dy, dfinal)
+    del tape
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    for _ in range(4):
+        _, _, tape = R.gated_scan(None, z, f, o, lens=lens, state=state, tape=True)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(20_000_000)
+            got = R.gated_scan_backward(None, tape, dy, dfinal)
+        made = [tape.states] + ([] if tape.lens is None else [tape.lens])
+        at, sizes = [t.data_ptr() for t in made], [t.numel() * t.element_size() for t in made]
+        del tape, made
+        # the side stream is not done with the states and the lengths: their memory is not anyone else's yet
+        new = [torch.full((n,), 255, dtype=torch.uint8, device="cuda") for n in sizes]
+        assert side.query() or not {t.data_ptr() for t in new} & set(at)
+        torch.cuda.current_stream().wait_stream(side)
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+            a.record_stream(torch.cuda.current_stream())
