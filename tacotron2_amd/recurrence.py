@@ -7,7 +7,7 @@ The gates do not depend on h, so a sequence is a scan that runs in parallel over
 [B, T, 3H] product need no copy).  fp32, bf16 and fp16; gates, state and sums are fp32, results are rounded once.
 
 ``ctx`` is a Context, an Engine, or None: torch's current stream on the tensors' device.  Nothing here synchronises, and every
-call can be captured into a graph (lengths on the host cannot: they have to be copied first)."""
+call can be captured into a graph (lengths on the host are refused there: they have to be copied first)."""
 from __future__ import annotations
 
 from typing import NamedTuple, Optional, Tuple
@@ -91,7 +91,12 @@ def _lengths(lens, B: int, T: int, device) -> Optional[torch.Tensor]:
     host = np.asarray(lens)
     if host.shape != (B,) or host.dtype.kind not in "iu" or (host < 0).any() or (host > T).any():
         raise ValueError(f"lens must be {B} whole numbers from 0 to {T}")
-    return torch.from_numpy(host.astype(np.int64)).to(device)
+    if torch.cuda.is_current_stream_capturing():
+        raise ValueError("lens on the host cannot be captured into a graph (the graph would keep this call's): copy them to the device first")
+    # through pinned memory: a copy out of any other waits for all the work in front of it
+    pinned = torch.empty(B, dtype=torch.int64, pin_memory=True)
+    pinned.numpy()[:] = host
+    return pinned.to(device, non_blocking=True)
 
 
 _NONE = (0, 0, 0)

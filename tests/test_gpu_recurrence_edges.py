@@ -4,8 +4,7 @@ import pytest
 
 pytestmark = pytest.mark.gpu
 
-from tests.test_gpu_recurrence import _check, _close, _inputs, _np
-from tests import recurrence_ref as ref
+from tests.test_gpu_recurrence import _check, _inputs
 
 torch = pytest.importorskip("torch")
 
@@ -120,3 +119,35 @@ def test_a_tape_used_on_another_stream_and_dropped_at_once(lens):
         for a, b in zip(got, want):
             assert torch.equal(a, b)
             a.record_stream(torch.cuda.current_stream())
+
+
+def test_lengths_on_the_host_do_not_wait_for_the_stream():
+    from tacotron2_amd import recurrence as R
+    z, f, o, state, dy, dfinal = _inputs(3, 300, 40, "f32", True, 2)
+    want = R.gated_scan(None, z, f, o, lens=torch.tensor([300, 17, 0], device="cuda"), state=state)
+    for lens in ([300, 17, 0], np.array([300, 17, 0], np.int32), torch.tensor([300, 17, 0])):
+        got = R.gated_scan(None, z, f, o, lens=lens, state=state)             # also: memory and code are there before the wait below
+        torch.cuda.synchronize()
+        torch.cuda._sleep(400_000_000)
+        busy = torch.cuda.Event()
+        busy.record()
+        got = R.gated_scan(None, z, f, o, lens=lens, state=state)
+        assert not busy.query(), "the call waited for what was queued before it"
+        if isinstance(lens, np.ndarray):
+            lens[:] = 1                                                        # the call has taken its lengths
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_lengths_on_the_host_are_refused_in_a_capture():
+    from tacotron2_amd import recurrence as R
+    z, f, o, state, _, _ = _inputs(2, 30, 40, "f32", True, 2)
+    want = R.gated_scan(None, z, f, o, lens=[30, 17], state=state)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(ValueError):
+            R.gated_scan(None, z, f, o, lens=[30, 17], state=state)
+        got = R.gated_scan(None, z, f, o, lens=None, state=state)
+    graph.replay()                                           # the refusal left the capture whole
+    torch.cuda.synchronize()
+    assert torch.equal(got[0][0], want[0][0]) and torch.equal(got[1], R.gated_scan(None, z, f, o, state=state)[1])
