@@ -574,7 +574,9 @@ static bool sizes_ok(int B, int T, int H) { return B >= 1 && B <= 65535 && T >= 
 
 extern "C" int64_t t2_gated_scan_tape(int B, int T, int H) {
     if (!sizes_ok(B, T, H)) return fail(T2_EINVAL, "bad shape [%d,%d,%d]", B, T, H);
-    return (int64_t)B * ((T + T2_SCAN_SPAN - 1) / T2_SCAN_SPAN) * H;
+    const int64_t rows = (int64_t)B * ((T + T2_SCAN_SPAN - 1) / T2_SCAN_SPAN);
+    if (rows > (INT64_MAX >> 3) / H) return fail(T2_EINVAL, "[%d,%d,%d] is too large", B, T, H);      // bytes of it are counted in 64 bits too
+    return rows * H;
 }
 
 // The tile of a call, by its sizes (kernel times in us; frames: B=32, T=800, H=512 bf16; long: B=2, T=65536, H=1024 bf16; odd: B=2,

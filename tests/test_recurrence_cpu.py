@@ -178,3 +178,9 @@ def test_context_options():
     assert lib.t2_ctx_set_option(ctx, b"scan_wait_us", 0) == _lib.T2_OK and lib.t2_ctx_set_option(ctx, b"scan_wait_us", 2000000) == _lib.T2_OK
     for bad in ((None, b"scan_wait_us", 1), (ctx, None, 1), (ctx, b"scan_wait", 1), (ctx, b"scan_wait_us", -1)):
         assert lib.t2_ctx_set_option(*bad) == _lib.T2_EINVAL, bad
+
+
+def test_sizes_whose_tape_has_no_count_are_refused():
+    lib = _lib.load()
+    assert lib.t2_gated_scan_tape(65535, 1 << 30, 1 << 24) < 0 and lib.t2_gated_scan_tape(1 << 14, 1 << 30, 1 << 24) < 0
+    assert lib.t2_gated_scan_tape(1 << 12, 1 << 30, 1 << 24) < 0 < lib.t2_gated_scan_tape(1 << 11, 1 << 30, 1 << 24) == 1 << 59 and lib.t2_gated_scan_ws(65535, 1 << 30, 1 << 24) < 0
