@@ -15,7 +15,6 @@ struct ElemF32 {
     static __device__ __forceinline__ float at(const Raw& r, int j) { return r[j]; }
     static __device__ __forceinline__ float get(const void* p, long long i) { return ((const float*)p)[i]; }
     static __device__ __forceinline__ void put(void* p, long long i, float v) { ((float*)p)[i] = v; }
-    static __device__ __forceinline__ void set(Raw& r, int j, float v) { r[j] = v; }
     static __device__ __forceinline__ Raw pack(float a, float b, float c, float d) { Raw r = {a, b, c, d}; return r; }
 };
 

@@ -434,7 +434,6 @@ __device__ __forceinline__ float gradients_again(int b, int len, int cc, int las
 }
 
 // the states in front of the pieces, from the tape's
-template <int TG, int L>
 __device__ __forceinline__ float tape_state(const t2_scan_args& a, int b, int first, int rows, int cc, int k) {
     const int ntape = (a.T + T2_SCAN_SPAN - 1) / T2_SCAN_SPAN;
     return cc >= 0 && k * T2_SCAN_SPAN < rows ? a.tape[((long long)b * ntape + first / T2_SCAN_SPAN + k) * a.H + cc] : 0.f;
@@ -444,7 +443,7 @@ __device__ __forceinline__ void distribute_states(const t2_scan_args& a, int b, 
     float h = 0.f;
 #pragma unroll
     for (int i = 0; i < TG; ++i) {
-        if (i * L % T2_SCAN_SPAN == 0) h = tape_state<TG, L>(a, b, first, rows, cc, i * L / T2_SCAN_SPAN);
+        if (i * L % T2_SCAN_SPAN == 0) h = tape_state(a, b, first, rows, cc, i * L / T2_SCAN_SPAN);
         const float2 p = piece[i][lane];
         ((float*)in[i])[lane] = h;
         h = fmaf(p.x, h, p.y);
