@@ -435,6 +435,7 @@ int t2_griffin_lim(t2_ctx* ctx, const float* spectrogram, int B, int T, int num_
  * For every row b and channel c, over the row's positions in order (from the last to the first where `reverse` is set):
  *     a = sigmoid(f_t)      h_t = a h_{t-1} + (1 - a) z_t      y_t = sigmoid(o_t) h_t   (y_t = h_t where o is NULL)
  * The recurrence is linear in h, so a whole sequence is a scan: it is split over the time axis, not run step by step.
+ *  - 1 <= B <= 65535, 1 <= T <= 2^30, 1 <= H <= 2^24.
  *  - z, f, o, y: [B][T][H] of one type, channels contiguous, strides in elements (any, 0 for inputs that are broadcast); o may be NULL.
  *  - lens: dev int64 [B] or NULL (all T).  Values outside [0, T] are taken as 0 and T.  Positions at or behind a row's length are not
  *    read into any result and give y = 0; a length of 0 leaves the state as it was.

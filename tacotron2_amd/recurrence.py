@@ -7,7 +7,11 @@ The gates do not depend on h, so a sequence is a scan that runs in parallel over
 [B, T, 3H] product need no copy).  fp32, bf16 and fp16; gates, state and sums are fp32, results are rounded once.
 
 ``ctx`` is a Context, an Engine, or None: torch's current stream on the tensors' device.  Nothing here synchronises, and every
-call can be captured into a graph (lengths on the host are refused there: they have to be copied first)."""
+call can be captured into a graph (lengths on the host are refused there: they have to be copied first).
+
+Like the rest of this package these calls are outside torch's autograd: results carry no history whatever their inputs require, and a
+state that is updated in place gets no new version.  ``gated_scan_backward`` gives the gradients; hand them on to whatever made z, f
+and o.  B is at most 65535, T 2^30, H 2^24, and a call at most 2^32 threads."""
 from __future__ import annotations
 
 from typing import NamedTuple, Optional, Tuple
