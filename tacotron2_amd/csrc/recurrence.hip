@@ -595,7 +595,7 @@ struct Tile {
 enum Shape { SHORT, MEDIUM, NARROW, WIDE, FEW };
 static constexpr Tile forward_tile[] = {{16, 8, 8}, {16, 32, 8}, {16, 16, 8}, {32, 8, 16}, {8, 32, 8}};
 static constexpr Tile backward_tile[] = {{16, 16, 4}, {16, 32, 8}, {16, 16, 4}, {32, 8, 8}, {8, 32, 8}};
-static constexpr int forward_waves[] = {4, 4, 4, 2, 4}, backward_waves[] = {3, 2, 3, 2, 2};     // a SIMD: registers for the tile without spills
+static constexpr int forward_waves[] = {4, 4, 4, 2, 4}, backward_waves[] = {3, 2, 3, 2, 2};     // a SIMD: registers for the tile without spills (but for 24 to 32 bytes a thread of forward fp32 tiles with an output gate)
 
 static Shape shape_of(bool backward, int B, int T, int H, bool buf) {
     const Tile* tiles = backward ? backward_tile : forward_tile;
