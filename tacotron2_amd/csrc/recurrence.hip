@@ -450,8 +450,9 @@ __device__ __forceinline__ void distribute_states(const t2_scan_args& a, int b, 
     }
 }
 
+// Returns the gradient that leaves the thread's first step for the state in front of it.
 template <typename E, bool GATE, bool BUF, bool NT, int LANES, int L, int C>
-__device__ __forceinline__ void back_finish(const t2_scan_args& a, const Place<BUF, LANES, L>& t, int first, int rows, const BackSteps<L>& s, const typename E::Raw* zr,
+__device__ __forceinline__ f32v4 back_finish(const t2_scan_args& a, const Place<BUF, LANES, L>& t, int first, int rows, const BackSteps<L>& s, const typename E::Raw* zr,
                                             const typename E::Raw* orr, const typename E::Raw* dr, f32v4 hin, f32v4 lin) {
     float h[4] = {hin[0], hin[1], hin[2], hin[3]}, d[4] = {lin[0], lin[1], lin[2], lin[3]};
     float wf[L][4], g[L][4];                                       // wf: df but for the gradient of h
@@ -488,6 +489,7 @@ __device__ __forceinline__ void back_finish(const t2_scan_args& a, const Place<B
         dz.template store<NT>(t.i0 + l, t.me.c, t.me.nc, t.i0 + l < rows && t.me.mine, z4[0], z4[1], z4[2], z4[3]);
         df.template store<NT>(t.i0 + l, t.me.c, t.me.nc, t.i0 + l < rows && t.me.mine, f4[0], f4[1], f4[2], f4[3]);
     }
+    return f32v4{d[0], d[1], d[2], d[3]};
 }
 
 template <typename E, bool GATE, bool BUF, int LANES, int L, int C>
@@ -497,7 +499,9 @@ __device__ __forceinline__ void back_zeros(const t2_scan_args& a, const Place<BU
     if (GATE) t.template zeros<E, C>(a.do_, first, a.T);
 }
 
-template <typename E, bool GATE, bool BUF, bool NT, int LANES, int TG, int L, int WAVES>
+// ONE: a sequence has one tile; nothing is drawn, published or looked back at, and the registers of that are free (B=64, T=250, H=2048 bf16:
+// 137 us with it, 129 so).  The forward kernel loses by the same cut (62 to 126: the compiler spills).
+template <typename E, bool GATE, bool BUF, bool NT, bool ONE, int LANES, int TG, int L, int WAVES>
 __global__ __launch_bounds__(LANES* TG, WAVES) void scan_tile_backward_kernel(t2_scan_args a, ScanWs w, int ntile) {
     constexpr int C = TG * L, CH = 4 * LANES;
     static_assert(C % T2_SCAN_SPAN == 0 && T2_SCAN_SPAN % L == 0, "tiles start where the tape has a state");
@@ -506,7 +510,7 @@ __global__ __launch_bounds__(LANES* TG, WAVES) void scan_tile_backward_kernel(t2
     __shared__ f32v4 s_h[TG][LANES], s_l[TG][LANES];
     const unsigned chains = gridDim.x / (unsigned)ntile, chain = chain_of(blockIdx.x, chains);
     const Place<BUF, LANES, L> t(a, chain);
-    const int tile = ntile - 1 - draw_tile(w, chain, ntile), first = tile * C;
+    const int tile = ONE ? 0 : ntile - 1 - draw_tile(w, chain, ntile), first = tile * C;
     if (first >= t.len && tile > 0) { back_zeros<E, GATE, BUF, LANES, L, C>(a, t, first); return; }
     const int rows = t.rows(first, C);
     Grads<E, L> in;
@@ -529,19 +533,27 @@ __global__ __launch_bounds__(LANES* TG, WAVES) void scan_tile_backward_kernel(t2
     } else if (threadIdx.x < 2 * CH) {
         const unsigned lane = threadIdx.x - CH;
         const int cc = channel_of<BUF>(t.c0, lane, a.H);
-        float At, Qt;
-        compose<TG, CH, true>(s_bwd, lane, At, Qt);
-        const int last = t.len > 0 ? (t.len - 1) / C : 0, at = last - tile;     // the last tile that is not all padding comes first
-        const long long line = (long long)chains * CH, place = (long long)chain * CH, slot = tile * line + place;
-        if (tile > 0) publish(w.piece + slot + lane, At, Qt);
         const float l0 = a.dfinal && cc >= 0 ? a.dfinal[(long long)t.b * a.H + cc] : 0.f;
-        const float l = look_back(w, at, l0, lane, slot, -line, at / SCAN_GROUP * line + place, line,
-                                  [&] { return gradients_again<E, GATE, TG, L>(t.b, t.len, cc, last, tile, l0); });
-        if (tile == 0 && a.dstate && cc >= 0) a.dstate[(long long)t.b * a.H + cc] = fmaf(At, l, Qt);
+        float l = l0;
+        if constexpr (!ONE) {
+            float At, Qt;
+            compose<TG, CH, true>(s_bwd, lane, At, Qt);
+            const int last = t.len > 0 ? (t.len - 1) / C : 0, at = last - tile;     // the last tile that is not all padding comes first
+            const long long line = (long long)chains * CH, place = (long long)chain * CH, slot = tile * line + place;
+            if (tile > 0) publish(w.piece + slot + lane, At, Qt);
+            l = look_back(w, at, l0, lane, slot, -line, at / SCAN_GROUP * line + place, line,
+                          [&] { return gradients_again<E, GATE, TG, L>(t.b, t.len, cc, last, tile, l0); });
+        }
         distribute<TG, CH, true>(s_bwd, s_l, lane, l);
     }
     __syncthreads();
-    back_finish<E, GATE, BUF, NT, LANES, L, C>(a, t, first, rows, s, in.z, in.o, in.d, s_h[t.tg][threadIdx.x % LANES], s_l[t.tg][threadIdx.x % LANES]);
+    const f32v4 d = back_finish<E, GATE, BUF, NT, LANES, L, C>(a, t, first, rows, s, in.z, in.o, in.d, s_h[t.tg][threadIdx.x % LANES], s_l[t.tg][threadIdx.x % LANES]);
+    // out of the steps themselves: where dfinal and dy cancel, the tile's composition has rounded its part already
+    if (tile == 0 && t.tg == 0 && a.dstate && t.me.mine) {
+        float* q = a.dstate + (long long)t.b * a.H + t.me.c;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) if (j < t.me.nc) q[j] = d[j];
+    }
     if (rows < C) back_zeros<E, GATE, BUF, LANES, L, C>(a, t, first);
 }
 
@@ -748,7 +760,7 @@ static int launch(t2_ctx* ctx, const t2_scan_args* a) {
         hipLaunchKernelGGL(scan_ws_kernel, dim3((unsigned)(nb < 2048 ? nb : 2048)), dim3(256), 0, ctx->stream, (uint4*)a->ws, blocks / ntile * 4, n16);
     }
     const dim3 grid((unsigned)blocks), threads(tile.lanes * tile.tg);
-    if constexpr (BACKWARD) hipLaunchKernelGGL((scan_tile_backward_kernel<E, GATE, BUF, NT, tile.lanes, tile.tg, tile.l, WAVES>), grid, threads, 0, ctx->stream, *a, w, ntile);
+    if constexpr (BACKWARD) hipLaunchKernelGGL((scan_tile_backward_kernel<E, GATE, BUF, NT, S != NARROW && S != WIDE, tile.lanes, tile.tg, tile.l, WAVES>), grid, threads, 0, ctx->stream, *a, w, ntile);
     else hipLaunchKernelGGL((scan_tile_kernel<E, GATE, BUF, NT, tile.lanes, tile.tg, tile.l, WAVES>), grid, threads, 0, ctx->stream, *a, w, ntile);
     HIP_TRY(hipGetLastError());
     return T2_OK;

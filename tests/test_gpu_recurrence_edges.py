@@ -151,3 +151,15 @@ def test_lengths_on_the_host_are_refused_in_a_capture():
     graph.replay()                                           # the refusal left the capture whole
     torch.cuda.synchronize()
     assert torch.equal(got[0][0], want[0][0]) and torch.equal(got[1], R.gated_scan(None, z, f, o, state=state)[1])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("T", [1, 2, 7, 140, 700])
+def test_gradients_that_cancel(dtype, T):
+    """dfinal next to -dy of the last step: what is left is as exact as the steps one after the other have it."""
+    z, f, _, state, dy, dfinal = _inputs(5, T, 140, dtype, False, T)
+    f[:, :-1] += 6.0                                                       # long memories: it reaches the first step
+    for reverse in (False, True):
+        last = dy[:, 0 if reverse else -1].float()
+        dfinal = -last * (1 + 2.0 ** -12 * torch.rand(5, 140, generator=torch.Generator().manual_seed(T)).cuda())
+        _check(z, f, None, None, state, dy, dfinal, reverse, dtype)
