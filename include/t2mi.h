@@ -453,7 +453,8 @@ int t2_griffin_lim(t2_ctx* ctx, const float* spectrogram, int B, int T, int num_
  *     active: dev uint8 [B] or NULL; rows where it is 0 keep their state and get y = 0.  y may be z, f or o itself; otherwise neither it nor
  *     the state may overlap another tensor.
  * An output (y, the gradients, final_state, dstate, the tape that is written, ws) that overlaps itself, an input (z, f, o, dy, lens, state, dfinal, the
- * tape that is read, active) or another output is refused, whatever the strides.
+ * tape that is read, active) or another output is refused, whatever the strides.  The rows of y and of the gradients have to be nested: all rows
+ * of one axis lie between two of the other's.
  * All three only enqueue; none allocates, so they can be captured.  Results do not depend on timing: tiles of a sequence wait for one
  * another for a bounded time (t2_ctx_set_option), and one whose wait ends computes the missing state itself. */
 #define T2_F32 0
